@@ -285,10 +285,11 @@ def _plain_context(s, name, layer):
 def _run_tree(s):
     if own:
         cache = s["cache"]
-        cache.invalidate_plan()  # a step has new lengths: its plan is made once, for all layers
+        # a step has new lengths: its plan is made once, for all layers
+        plan = cache.plan_tree(s["q"].shape[2], s["q"].shape[3], s["n_draft"])
         for layer in range(s["q"].shape[0]):
-            cache.attend_tree(layer, s["q"][layer], s["k"][layer], s["v"][layer], mask=s["mask"],
-                              n_draft=s["n_draft"], out=s["out"][layer])
+            cache.attend_tree(layer, s["q"][layer], s["k"][layer], s["v"][layer], mask=s["mask"], plan=plan,
+                              out=s["out"][layer])
         return s["out"]
     L, B, T, hq, d = s["q"].shape
     P, hkv = s["staging_k"].shape[2:4]
