@@ -172,7 +172,7 @@ typedef struct mg_layer_ptrs {
 typedef struct mg_allocator {
     int32_t* free_stack; /* [N] */
     int32_t* n_free;     /* [1] */
-    int32_t* in_use;     /* [N] 1 while allocated */
+    int32_t* in_use;     /* [N] sequences that hold the page (0: free; above 1 only after mg_fork_sequences) */
     int64_t num_pages;
 } mg_allocator;
 
@@ -347,7 +347,9 @@ MG_API mg_status mg_gather_dequant(const mg_cache_layout* layout, const mg_layer
 /* Free every page of the listed sequences back to the allocator (pages in
  * block-table order, sequences in list order -- the order in which the
  * reference's BlockAllocator.free would be called) and set their seq_lens to
- * 0.  A page already free sets MG_DEV_DOUBLE_FREE and is skipped. */
+ * 0.  A page that other sequences hold too (mg_fork_sequences) loses one
+ * holder and goes back with its last one.  A page already free sets
+ * MG_DEV_DOUBLE_FREE and is skipped. */
 MG_API mg_status mg_free_sequences(const mg_allocator* alloc, const int32_t* block_tables,
                                    int32_t max_blocks, int32_t* seq_lens, int32_t batch,
                                    const int32_t* seq_ids, int32_t num_seqs, int32_t page_size,
@@ -364,6 +366,81 @@ MG_API mg_status mg_truncate_sequences(const mg_allocator* alloc, const int32_t*
                                        const int32_t* seq_ids, const int32_t* new_lens,
                                        int32_t num_seqs, int32_t page_size, int32_t* dev_status,
                                        mg_stream_t stream);
+
+/* Make sequence dst_ids[i] a copy of sequence src_ids[i], whole (new_lens
+ * NULL) or its first new_lens[i] tokens, in every layer.  Committed pages are
+ * shared (they are never written again): the target's block-table entries
+ * become the source's and each page counts one more holder.  The exact rows
+ * after them are copied into the target's staging rows; where the new length
+ * cuts a committed page, that page's rows are dequantized (code * scale,
+ * rounded once to the staging type) instead.  What a target held before is
+ * released first, in list order, as mg_free_sequences would.
+ * layer0 holds layer 0's pointers; the buffers of layer i follow at i times
+ * their size (staging [num_layers, batch, P, Hkv, D]).  A pair whose ids or
+ * length are out of range, whose source is its target, or whose target is
+ * also a source or an earlier pair's target, sets MG_DEV_BAD_ARGUMENT and is
+ * skipped.  workspace: mg_fork_workspace_bytes() bytes, 4-byte aligned, the
+ * first 8 zero before the first call (every call leaves them zero); calls that
+ * share it must not overlap on the device.  No counterpart in the reference. */
+MG_API int64_t mg_fork_workspace_bytes(int32_t num_pairs);
+MG_API mg_status mg_fork_sequences(const mg_allocator* alloc, const mg_cache_layout* layout,
+                                   const mg_layer_ptrs* layer0, int32_t num_layers, int32_t* block_tables,
+                                   int32_t* seq_lens, int32_t batch, const int32_t* src_ids, const int32_t* dst_ids,
+                                   const int32_t* new_lens, int32_t num_pairs, void* workspace,
+                                   int64_t workspace_bytes, int32_t* dev_status, mg_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of drafted tokens over the cache.  No counterpart in the reference
+ * (one decode query per head and call, csrc/bindings.cpp:82-106).
+ *
+ * Every sequence b has up to max_draft tokens that are not in its cache yet
+ * (a tree or chain of drafted tokens to verify, a chunk of a prompt).  Token t
+ * attends to the whole cached context and to those drafted tokens u that the
+ * mask lets it see:
+ *   out[b, t, h] = sum_j p_j v_j,  p = softmax_j(scale * q[b, t, h] . k_j)
+ * A token that sees nothing (empty context, empty mask row) gets zeros, and so
+ * do the rows t >= n_draft[b].  Keys that are masked out do not take part,
+ * whatever their values (infinities and NaN included).  The cache is read,
+ * not changed: accepted tokens are appended afterwards (mg_kv_append).
+ * ---------------------------------------------------------------------- */
+typedef struct mg_tree_draft {
+    const void* q; /* fp16 [batch, max_draft, num_q_heads, D], strides in elements, D contiguous */
+    const void* k; /* fp16 [batch, max_draft, Hkv, D] */
+    const void* v; /* fp16 [batch, max_draft, Hkv, D] */
+    int64_t q_stride[3]; /* sequence, token, head; multiples of 4 elements */
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    const void* mask;    /* one byte per (t, u), nonzero = t sees u: [max_draft, max_draft] rows; NULL: u <= t */
+    int64_t mask_stride; /* bytes from one sequence's mask to the next; 0: one mask for all */
+    int32_t max_draft;
+    int32_t num_q_heads;
+} mg_tree_draft;
+
+/* The step's plan: how the work is split over the GPU.  It depends on the
+ * lengths only, so one plan serves every layer; it is rebuilt when seq_lens,
+ * n_draft (int32 [batch], NULL: all max_draft) or the shapes change.  plan:
+ * mg_tree_plan_bytes() bytes of device memory, 16-byte aligned.  A negative
+ * or too large length or count sets MG_DEV_BAD_ARGUMENT and plans that
+ * sequence as empty (its rows become zeros).  Both byte counts are 0 for an
+ * unsupported shape (mg_last_error says why). */
+MG_API int64_t mg_tree_plan_bytes(const mg_cache_layout* layout, int32_t batch, int32_t max_draft,
+                                  int32_t num_q_heads);
+MG_API int64_t mg_tree_workspace_bytes(const mg_cache_layout* layout, int32_t batch, int32_t max_draft,
+                                       int32_t num_q_heads);
+MG_API mg_status mg_tree_plan(const mg_cache_layout* layout, const int32_t* seq_lens, const int32_t* n_draft,
+                              int32_t batch, int32_t max_draft, int32_t num_q_heads, void* plan, int64_t plan_bytes,
+                              int32_t* dev_status, mg_stream_t stream);
+
+/* The attention of one layer.  fp16 staging; head_dim 64 or 128; out fp16
+ * [batch, max_draft, num_q_heads, D].  workspace: mg_tree_workspace_bytes()
+ * bytes, 16-byte aligned, no initial contents; calls that share one must not
+ * overlap on the device.  A plan made for other shapes sets
+ * MG_DEV_BAD_ARGUMENT and writes nothing; after a refused step (the stop bits
+ * of mg_plan_append) the call does nothing. */
+MG_API mg_status mg_tree_attention(const mg_cache_layout* layout, const mg_layer_ptrs* layer,
+                                   const int32_t* block_tables, int32_t batch, const mg_tree_draft* draft,
+                                   const void* plan, int64_t plan_bytes, float scale, void* out, void* workspace,
+                                   int64_t workspace_bytes, int32_t* dev_status, mg_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Dense-side helpers of a Llama decode step (fp16 storage, fp32 math).  No
@@ -383,6 +460,20 @@ MG_API mg_status mg_rmsnorm_f16(const void* x, const void* w, void* y, int64_t r
 MG_API mg_status mg_rope_qkv_f16(const void* qkv, const int64_t* pos, const float* cos_table,
                                  const float* sin_table, void* q, void* k, void* v, int32_t batch,
                                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, mg_stream_t stream);
+
+/* For models that normalise q and k per head: rows of a fused projection
+ * qkv [rows, (Hq + 2 Hkv) * D] (q | k | v heads, row_stride elements apart) ->
+ * q [rows, Hq, D] and k [rows, Hkv, D], each head RMS-normalised over its D
+ * values (weights q_weight / k_weight [D]) and rotated (rotate-half) at pos[r]
+ * by cos / sin [table_rows, D / 2], in fp32 with one rounding; v [rows, Hkv, D]
+ * copied, or NULL to leave it in the projection.  Any even D.  The q and k of a
+ * row whose position is outside the tables become zeros and set
+ * MG_DEV_BAD_ARGUMENT in *dev_status (nullable). */
+MG_API mg_status mg_qk_norm_rope_f16(const void* qkv, int64_t row_stride, const void* q_weight, const void* k_weight,
+                                     const int64_t* pos, const float* cos_table, const float* sin_table,
+                                     int64_t table_rows, float eps, void* q, void* k, void* v, int64_t rows,
+                                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     int32_t* dev_status, mg_stream_t stream);
 
 /* h[r, j] = fp16(silu(gu[r, j])) * gu[r, ffn + j], gu [rows, 2 ffn]. */
 MG_API mg_status mg_silu_mul_f16(const void* gu, void* h, int64_t rows, int64_t ffn, mg_stream_t stream);

@@ -24,6 +24,12 @@ A decode/prefill step is:
   for layer: cache.append(layer, k, v) # quantize filled pages, stage the rest
              out = cache.attend(layer, q)
 
+Several tokens per sequence against the cache (drafted tokens to verify, a
+chunk of a prompt), and sequences that share pages:
+  plan = cache.plan_tree(T, num_q_heads)       # once per step, for all layers
+  out = cache.attend_tree(layer, q, k, v, plan=plan, mask=mask)
+  cache.fork(src, dst)                         # dst become copies of src
+
 The first ``attend`` after the lengths or block tables change (begin_step,
 truncate, free, reset) builds the step's decode plan -- the split of the
 batch's pages over the SMs, with a copy of each CTA's first page ids -- and
@@ -33,6 +39,7 @@ the other layers reuse it.  Code that writes ``seq_lens`` or
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 
 import torch
 
@@ -55,6 +62,19 @@ def _get_C():
     from . import _C
 
     return _C
+
+
+@dataclass(frozen=True)
+class TreePlan:
+    """How a step's drafted-token attention is split over the GPU, and the
+    workspace its calls share (so they run on one stream)."""
+
+    buf: torch.Tensor
+    nbytes: int
+    max_draft: int
+    num_q_heads: int
+    cache: object
+    version: int
 
 
 class BatchedPagedKVCache:
@@ -107,6 +127,8 @@ class BatchedPagedKVCache:
         self._plan = None
         self._plan_ok = False
         self._plan_last = False  # the plan kernel is the cache's latest launch (nothing after it yet)
+        self._lens_version = 0  # changes with the lengths or tables; a TreePlan of another version is stale
+        self._fork_ws = torch.zeros(2, dtype=torch.int32, device=self.device)
 
     # ------------------------------------------------------------------ steps
     def begin_step(self, n_new, plan: bool = False) -> None:
@@ -114,6 +136,7 @@ class BatchedPagedKVCache:
         plan=True also builds the step's decode plan, in the same launch (mg_plan_step): call it so
         before the step's first append, and every attention launch of the step reads its plan early."""
         C = _get_C()
+        self._lens_version += 1
         if isinstance(n_new, int):
             if n_new < 0:
                 raise ValueError("n_new must be >= 0")
@@ -177,6 +200,7 @@ class BatchedPagedKVCache:
     def invalidate_plan(self) -> None:
         """Mark the decode plan stale (after writing seq_lens or block_tables directly)."""
         self._plan_ok = False
+        self._lens_version += 1
 
     def prepare_plan(self) -> None:
         """Build the step's decode plan now if the lengths changed since the last
@@ -231,6 +255,92 @@ class BatchedPagedKVCache:
         self._plan_last = False
         return out
 
+    # ------------------------------------------------- drafted and forked sequences
+    def plan_tree(self, max_draft: int, num_q_heads: int, n_draft: torch.Tensor | None = None) -> TreePlan:
+        """The plan of a step's ``attend_tree`` calls: up to max_draft drafted tokens per
+        sequence (n_draft int32 [B]: how many each has; all max_draft without it).  It holds
+        until the lengths change (begin_step, truncate, fork, ...), for every layer."""
+        if max_draft < 0:
+            raise ValueError(f"max_draft must be >= 0, got {max_draft}")
+        if num_q_heads <= 0 or num_q_heads % self.num_kv_heads:
+            raise ValueError(f"num_q_heads={num_q_heads} must be divisible by num_kv_heads={self.num_kv_heads}")
+        if self.staging_dtype != torch.float16:
+            raise ValueError("drafted-token attention needs a cache with float16 staging")
+        if n_draft is not None:
+            n_draft = torch.as_tensor(n_draft, dtype=torch.int32, device=self.device).contiguous()
+            if n_draft.shape != (self.batch,):
+                raise ValueError(f"n_draft must have one entry per sequence ({self.batch}), got {tuple(n_draft.shape)}")
+        buf, nbytes = _get_C().tree_plan(self.k_pool, self.block_tables, self.seq_lens, max_draft, num_q_heads, n_draft,
+                                         self.status)
+        return TreePlan(buf, nbytes, max_draft, num_q_heads, self, self._lens_version)
+
+    def attend_tree(self, layer: int, q: torch.Tensor, k_draft: torch.Tensor, v_draft: torch.Tensor,
+                    mask: torch.Tensor | None = None, n_draft: torch.Tensor | None = None,
+                    plan: TreePlan | None = None, scale: float | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of T drafted tokens per sequence over its cached context and each other.
+
+        q [B, T, Hq, D], k_draft / v_draft [B, T, Hkv, D] fp16 (any strides with a contiguous
+        last dimension).  mask bool [T, T] or [B, T, T]: True where token t sees drafted token
+        u (``tree.tree_mask`` makes one from parents); without it token t sees u <= t, as in a
+        chunk of a prompt.  n_draft int32 [B]: drafted tokens of each sequence; later rows come
+        out as zeros, as does a row that sees nothing.  The cache is not changed: append the
+        accepted tokens afterwards.  plan: ``plan_tree``'s, shared by the layers of a step
+        (which then carries n_draft); without it the call makes its own."""
+        if q.dim() != 4 or q.shape[0] != self.batch or q.shape[3] != self.head_dim:
+            raise ValueError(f"q must be [{self.batch}, drafted tokens, num_q_heads, {self.head_dim}], "
+                             f"got {tuple(q.shape)}")
+        T, hq = q.shape[1], q.shape[2]
+        if plan is None:
+            plan = self.plan_tree(T, hq, n_draft)
+        else:
+            if n_draft is not None:
+                raise ValueError("n_draft belongs to the plan: give it to plan_tree")
+            if plan.cache is not self or plan.max_draft != T or plan.num_q_heads != hq:
+                raise ValueError("the plan was made for another cache, number of drafted tokens or of q heads")
+            if plan.version != self._lens_version:
+                raise ValueError("the plan is stale: lengths or block tables changed after plan_tree")
+        sc = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
+        if not (sc > 0 and math.isfinite(sc)):
+            raise ValueError(f"scale must be a positive finite number, got {scale}")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _get_C().tree_attention(q, k_draft, v_draft, mask, self.k_pool, self.v_pool, self.k_scales, self.v_scales,
+                                self.staging_k, self.staging_v, self.block_tables, layer, plan.buf, plan.nbytes, sc,
+                                out, self.status)
+        self._plan_last = False
+        return out
+
+    def fork(self, src, dst, lens=None) -> None:
+        """Sequence dst[i] becomes a copy of sequence src[i] (or of its first lens[i] tokens)
+        in every layer: samples of one prompt, beams, a shared prefix.
+
+        Committed pages are shared and go back to the pool with their last holder; the exact
+        rows after them are copied, or dequantized where lens cuts a committed page.  What dst
+        held is released first.  src, dst, lens: lists or int32 tensors; a target may not be a
+        source or appear twice (device tensors: such pairs are skipped and ``check`` raises)."""
+        if not any(isinstance(x, torch.Tensor) and x.is_cuda for x in (src, dst)):
+            s, d = (torch.as_tensor(x).flatten().tolist() for x in (src, dst))
+            if len(s) != len(d):
+                raise ValueError("src and dst must have the same length")
+            if any(not 0 <= x < self.batch for x in s + d):
+                raise ValueError(f"sequence ids must be in [0, {self.batch})")
+            if len(set(d)) != len(d) or set(d) & set(s):
+                raise ValueError("a target may not be a source or appear twice")
+        ids = [torch.as_tensor(x, dtype=torch.int32).to(self.device).contiguous() for x in (src, dst)]
+        if lens is not None:
+            lens = torch.as_tensor(lens, dtype=torch.int32).to(self.device).contiguous()
+        C = _get_C()
+        need = C.fork_workspace_bytes(ids[0].numel()) // 4
+        if need > self._fork_ws.numel():
+            self._fork_ws = torch.zeros(need, dtype=torch.int32, device=self.device)
+        self._plan_ok = False
+        self._lens_version += 1
+        C.fork_sequences(self.allocator.free_stack, self.allocator.n_free, self.allocator.in_use, self.k_pool,
+                         self.v_pool, self.k_scales, self.v_scales, self.staging_k, self.staging_v, self.block_tables,
+                         self.seq_lens, ids[0], ids[1], lens, self._fork_ws, self.status)
+        self._plan_last = False
+
     def gather(self, layer: int, dtype=torch.float32, include_staging: bool = True):
         """Dequantized K, V of every sequence, packed: ([total, Hkv, D], [total, Hkv, D], cu_seqlens [B+1])."""
         lens = self.seq_lens.to("cpu")
@@ -252,6 +362,7 @@ class BatchedPagedKVCache:
         """Return every page of the given sequences to the pool and reset them to length 0."""
         ids = torch.as_tensor(seq_ids, dtype=torch.int32).to(self.device)
         self._plan_ok = False
+        self._lens_version += 1
         _get_C().free_sequences(self.allocator.free_stack, self.allocator.n_free, self.allocator.in_use,
                                 self.block_tables, self.seq_lens, ids, self.page_size, self.status)
 
@@ -268,6 +379,7 @@ class BatchedPagedKVCache:
         else:
             nl = torch.as_tensor(new_lens, dtype=torch.int32)
         self._plan_ok = False
+        self._lens_version += 1
         _get_C().truncate_sequences(self.allocator.free_stack, self.allocator.n_free, self.allocator.in_use,
                                     self.block_tables, self.seq_lens, ids.to(self.device), nl.to(self.device),
                                     self.page_size, self.status)
@@ -279,6 +391,7 @@ class BatchedPagedKVCache:
         self.status.zero_()
         self._max_len = 0
         self._plan_ok = False
+        self._lens_version += 1
 
     # ------------------------------------------------------------- inspection
     def check(self) -> None:
@@ -344,7 +457,7 @@ class DecodeGraph:
         self.graph.replay()
         self.cache._max_len = min(self.cache._max_len + self.n_new,
                                   self.cache.max_blocks * self.cache.page_size + self.cache.page_size - 1)
-        self.cache._plan_ok = False  # lengths moved on the device
+        self.cache.invalidate_plan()  # lengths moved on the device
 
 
 def paged_decode_attention(cache: BatchedPagedKVCache, layer: int, q: torch.Tensor, scale=None, out=None):

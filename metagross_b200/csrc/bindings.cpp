@@ -581,6 +581,199 @@ void gather_dequant(torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor k_
                  "gather_dequant");
 }
 
+// ---------------------------------------------------------------------------
+// drafted and forked sequences.  These take the cache's whole [L, ...] tensors
+// and a layer index, so that a call builds no per-layer views.
+// ---------------------------------------------------------------------------
+
+struct LayerSet {
+    mg_cache_layout L;
+    mg_layer_ptrs ptrs;  // of the chosen layer
+    int64_t layers, batch;
+};
+
+LayerSet make_layers(const torch::Tensor& k_pool, const torch::Tensor& v_pool, const torch::Tensor& k_scales,
+                     const torch::Tensor& v_scales, const torch::Tensor& staging_k, const torch::Tensor& staging_v,
+                     const torch::Tensor& block_tables, int64_t layer) {
+    TORCH_CHECK(k_pool.is_cuda() && v_pool.is_cuda() && k_scales.is_cuda() && v_scales.is_cuda() &&
+                    staging_k.is_cuda() && staging_v.is_cuda() && block_tables.is_cuda(),
+                "the cache's tensors must be CUDA tensors");
+    const bool i4 = k_pool.scalar_type() == torch::kUInt8;
+    TORCH_CHECK(k_pool.dim() == 5 && v_pool.sizes() == k_pool.sizes() && k_pool.is_contiguous() &&
+                    v_pool.is_contiguous() && (i4 || k_pool.scalar_type() == torch::kInt8) &&
+                    v_pool.scalar_type() == k_pool.scalar_type(),
+                "pools must be equal contiguous int8 or uint8 tensors [layers, num_pages, page_size, num_kv_heads, row]");
+    const int64_t layers = k_pool.size(0), N = k_pool.size(1), P = k_pool.size(2), H = k_pool.size(3);
+    const int64_t D = i4 ? k_pool.size(4) * 2 : k_pool.size(4);
+    TORCH_CHECK(layer >= 0 && layer < layers, "layer ", layer, " is out of range [0, ", layers, ")");
+    const bool th = k_scales.dim() == 4;
+    TORCH_CHECK(k_scales.scalar_type() == torch::kFloat32 && v_scales.scalar_type() == torch::kFloat32 &&
+                    k_scales.is_contiguous() && v_scales.is_contiguous() && v_scales.sizes() == k_scales.sizes() &&
+                    k_scales.dim() == (th ? 4 : 2) && k_scales.size(0) == layers && k_scales.size(1) == N &&
+                    (!th || (k_scales.size(2) == P && k_scales.size(3) == H)),
+                "scales must be contiguous float32 [layers, num_pages] or [layers, num_pages, page_size, num_kv_heads]");
+    TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && block_tables.dim() == 2 && block_tables.is_contiguous(),
+                "block_tables must be a contiguous int32 [batch, max_blocks] tensor");
+    const int64_t B = block_tables.size(0);
+    TORCH_CHECK(staging_k.dim() == 5 && staging_v.sizes() == staging_k.sizes() && staging_k.is_contiguous() &&
+                    staging_v.is_contiguous() && staging_v.scalar_type() == staging_k.scalar_type() &&
+                    staging_k.size(0) == layers && staging_k.size(1) == B && staging_k.size(2) == P &&
+                    staging_k.size(3) == H && staging_k.size(4) == D,
+                "staging must be contiguous [layers, batch, page_size, num_kv_heads, head_dim]");
+    LayerSet s{};
+    s.L.kv_dtype = i4 ? MG_KV_INT4 : MG_KV_INT8;
+    s.L.staging_dtype = float_code(staging_k, "staging");
+    s.L.page_size = static_cast<int32_t>(P);
+    s.L.num_kv_heads = static_cast<int32_t>(H);
+    s.L.head_dim = static_cast<int32_t>(D);
+    s.L.max_blocks = static_cast<int32_t>(block_tables.size(1));
+    s.L.num_pages = N;
+    s.L.scale_layout = th ? MG_SCALE_TOKEN_HEAD : MG_SCALE_PAGE;
+    s.layers = layers;
+    s.batch = B;
+    auto at = [&](const torch::Tensor& t) {
+        return static_cast<char*>(t.data_ptr()) + t.stride(0) * layer * static_cast<int64_t>(t.element_size());
+    };
+    s.ptrs.k_pool = at(k_pool);
+    s.ptrs.v_pool = at(v_pool);
+    s.ptrs.k_scales = reinterpret_cast<float*>(at(k_scales));
+    s.ptrs.v_scales = reinterpret_cast<float*>(at(v_scales));
+    s.ptrs.staging_k = at(staging_k);
+    s.ptrs.staging_v = at(staging_v);
+    return s;
+}
+
+mg_cache_layout tree_layout(const torch::Tensor& k_pool, const torch::Tensor& block_tables) {
+    TORCH_CHECK(k_pool.dim() == 5 && block_tables.dim() == 2, "k_pool must be 5-D and block_tables 2-D");
+    mg_cache_layout L{};
+    const bool i4 = k_pool.scalar_type() == torch::kUInt8;
+    L.kv_dtype = i4 ? MG_KV_INT4 : MG_KV_INT8;
+    L.staging_dtype = MG_F16;
+    L.page_size = static_cast<int32_t>(k_pool.size(2));
+    L.num_kv_heads = static_cast<int32_t>(k_pool.size(3));
+    L.head_dim = static_cast<int32_t>(i4 ? k_pool.size(4) * 2 : k_pool.size(4));
+    L.max_blocks = static_cast<int32_t>(block_tables.size(1));
+    L.num_pages = k_pool.size(1);
+    return L;
+}
+
+int32_t to_i32(int64_t v, const char* what) {
+    TORCH_CHECK(v >= 0 && v <= std::numeric_limits<int32_t>::max(), what, " must be in [0, 2^31), got ", v);
+    return static_cast<int32_t>(v);
+}
+
+// The step's plan and the workspace of its attention calls, as one uint8
+// tensor: the plan's bytes (a multiple of 16), then the workspace's.
+std::tuple<torch::Tensor, int64_t> tree_plan(torch::Tensor k_pool, torch::Tensor block_tables, torch::Tensor seq_lens,
+                                             int64_t max_draft, int64_t num_q_heads,
+                                             c10::optional<torch::Tensor> n_draft,
+                                             c10::optional<torch::Tensor> status) {
+    TORCH_CHECK(k_pool.is_cuda(), "k_pool must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(k_pool.device());
+    const auto L = tree_layout(k_pool, block_tables);
+    const int32_t B = to_i32(block_tables.size(0), "batch"), T = to_i32(max_draft, "max_draft"),
+                  Hq = to_i32(num_q_heads, "num_q_heads");
+    check_i32_vec(seq_lens, B, "seq_lens");
+    const int32_t* nd = nullptr;
+    if (n_draft.has_value() && n_draft->defined()) {
+        check_i32_vec(*n_draft, B, "n_draft");
+        TORCH_CHECK(n_draft->numel() == B, "n_draft must have one entry per sequence");
+        nd = n_draft->data_ptr<int32_t>();
+    }
+    const int64_t pb = mg_tree_plan_bytes(&L, B, T, Hq), wb = mg_tree_workspace_bytes(&L, B, T, Hq);
+    TORCH_CHECK(pb > 0 && wb > 0, "tree_plan: ", mg_last_error());
+    const int64_t at = (pb + 255) / 256 * 256;
+    auto buf = torch::empty({at + wb}, torch::TensorOptions().dtype(torch::kUInt8).device(k_pool.device()));
+    check_status(mg_tree_plan(&L, seq_lens.data_ptr<int32_t>(), nd, B, T, Hq, buf.data_ptr(), at, status_ptr(status),
+                              cur_stream()),
+                 "tree_plan");
+    return std::make_tuple(buf, at);
+}
+
+void draft_strides(const torch::Tensor& t, int64_t B, int64_t T, int64_t H, int64_t D, const char* what,
+                   const void** ptr, int64_t (&stride)[3]) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kHalf && t.dim() == 4 && t.size(0) == B && t.size(1) == T &&
+                    t.size(2) == H && t.size(3) == D,
+                what, " must be a float16 CUDA tensor [", B, ", ", T, ", ", H, ", ", D, "]");
+    TORCH_CHECK(t.stride(3) == 1, what, "'s last dimension must be contiguous");
+    for (int i = 0; i < 3; ++i) {
+        stride[i] = t.size(i) == 1 ? 0 : t.stride(i);
+        TORCH_CHECK(stride[i] % 4 == 0, what, "'s strides must be multiples of 4 elements");
+    }
+    *ptr = t.data_ptr();
+    TORCH_CHECK((reinterpret_cast<uintptr_t>(*ptr) & 7u) == 0, what, " must start on 8 bytes");
+}
+
+void tree_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> mask,
+                    torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor k_scales, torch::Tensor v_scales,
+                    torch::Tensor staging_k, torch::Tensor staging_v, torch::Tensor block_tables, int64_t layer,
+                    torch::Tensor plan, int64_t plan_bytes, double scale, torch::Tensor out,
+                    c10::optional<torch::Tensor> status) {
+    TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(q.device());
+    auto s = make_layers(k_pool, v_pool, k_scales, v_scales, staging_k, staging_v, block_tables, layer);
+    TORCH_CHECK(q.dim() == 4, "q must be [batch, drafted tokens, num_q_heads, head_dim]");
+    const int64_t B = s.batch, T = q.size(1), Hq = q.size(2), H = s.L.num_kv_heads, D = s.L.head_dim;
+    mg_tree_draft d{};
+    draft_strides(q, B, T, Hq, D, "q", &d.q, d.q_stride);
+    draft_strides(k, B, T, H, D, "k_draft", &d.k, d.k_stride);
+    draft_strides(v, B, T, H, D, "v_draft", &d.v, d.v_stride);
+    d.max_draft = to_i32(T, "drafted tokens");
+    d.num_q_heads = to_i32(Hq, "num_q_heads");
+    if (mask.has_value() && mask->defined()) {
+        const auto& m = *mask;
+        const bool one = m.dim() == 2;
+        TORCH_CHECK(m.is_cuda() && m.scalar_type() == torch::kBool && (one || (m.dim() == 3 && m.size(0) == B)) &&
+                        m.size(-1) == T && m.size(-2) == T,
+                    "mask must be a bool CUDA tensor [", T, ", ", T, "] or [", B, ", ", T, ", ", T, "]");
+        TORCH_CHECK((T <= 1 || (m.stride(-1) == 1 && m.stride(-2) == T)), "the mask's rows must be contiguous");
+        d.mask = m.data_ptr();
+        d.mask_stride = one || B == 1 ? 0 : m.stride(0);
+    }
+    TORCH_CHECK(out.is_cuda() && out.scalar_type() == torch::kHalf && out.is_contiguous() && out.sizes() == q.sizes(),
+                "out must be a contiguous float16 CUDA tensor shaped like q");
+    TORCH_CHECK(std::isfinite(scale) && scale > 0.0, "attention scale must be positive and finite, got ", scale);
+    TORCH_CHECK(plan.is_cuda() && plan.is_contiguous() && plan.scalar_type() == torch::kUInt8 && plan_bytes >= 0 &&
+                    plan_bytes <= plan.numel() && plan_bytes % 16 == 0,
+                "plan must be the tensor that tree_plan made");
+    char* base = static_cast<char*>(plan.data_ptr());
+    check_status(mg_tree_attention(&s.L, &s.ptrs, block_tables.data_ptr<int32_t>(), static_cast<int32_t>(B), &d, base,
+                                   plan_bytes, static_cast<float>(scale), out.data_ptr(), base + plan_bytes,
+                                   plan.numel() - plan_bytes, status_ptr(status), cur_stream()),
+                 "tree_attention");
+}
+
+int64_t fork_workspace_bytes(int64_t num_pairs) { return mg_fork_workspace_bytes(to_i32(num_pairs, "num_pairs")); }
+
+void fork_sequences(torch::Tensor free_stack, torch::Tensor n_free, torch::Tensor in_use, torch::Tensor k_pool,
+                    torch::Tensor v_pool, torch::Tensor k_scales, torch::Tensor v_scales, torch::Tensor staging_k,
+                    torch::Tensor staging_v, torch::Tensor block_tables, torch::Tensor seq_lens, torch::Tensor src_ids,
+                    torch::Tensor dst_ids, c10::optional<torch::Tensor> new_lens, torch::Tensor workspace,
+                    c10::optional<torch::Tensor> status) {
+    TORCH_CHECK(k_pool.is_cuda(), "k_pool must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(k_pool.device());
+    auto a = make_alloc(free_stack, n_free, in_use);
+    auto s = make_layers(k_pool, v_pool, k_scales, v_scales, staging_k, staging_v, block_tables, 0);
+    check_i32_vec(seq_lens, s.batch, "seq_lens");
+    const int64_t n = src_ids.numel();
+    check_i32_vec(src_ids, n, "src_ids");
+    check_i32_vec(dst_ids, n, "dst_ids");
+    TORCH_CHECK(dst_ids.numel() == n, "src_ids and dst_ids must have the same length");
+    const int32_t* lens = nullptr;
+    if (new_lens.has_value() && new_lens->defined()) {
+        TORCH_CHECK(new_lens->numel() == n, "new_lens must have one entry per pair");
+        check_i32_vec(*new_lens, n, "new_lens");
+        lens = new_lens->data_ptr<int32_t>();
+    }
+    check_i32_vec(workspace, 2, "workspace");
+    check_status(mg_fork_sequences(&a, &s.L, &s.ptrs, static_cast<int32_t>(s.layers), block_tables.data_ptr<int32_t>(),
+                                   seq_lens.data_ptr<int32_t>(), static_cast<int32_t>(s.batch),
+                                   src_ids.data_ptr<int32_t>(), dst_ids.data_ptr<int32_t>(), lens,
+                                   to_i32(n, "pairs"), workspace.data_ptr(), workspace.numel() * 4,
+                                   status_ptr(status), cur_stream()),
+                 "fork_sequences");
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -626,6 +819,45 @@ void rope_qkv(torch::Tensor qkv, torch::Tensor pos, torch::Tensor cos_table, tor
                                  static_cast<int32_t>(B), static_cast<int32_t>(Hq), static_cast<int32_t>(Hkv),
                                  static_cast<int32_t>(D), cur_stream()),
                  "rope_qkv");
+}
+
+void qk_norm_rope(torch::Tensor qkv, torch::Tensor q_weight, torch::Tensor k_weight, torch::Tensor pos,
+                  torch::Tensor cos_table, torch::Tensor sin_table, double eps, torch::Tensor q, torch::Tensor k,
+                  c10::optional<torch::Tensor> v, c10::optional<torch::Tensor> status) {
+    TORCH_CHECK(qkv.is_cuda(), "qkv must be a CUDA tensor");
+    const c10::cuda::CUDAGuard guard(qkv.device());
+    check_f16_cuda(q, "q");
+    check_f16_cuda(k, "k");
+    check_f16_cuda(q_weight, "q_weight");
+    check_f16_cuda(k_weight, "k_weight");
+    TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && k.size(0) == q.size(0) && k.size(2) == q.size(2),
+                "q must be [rows, Hq, D] and k [rows, Hkv, D]");
+    const int64_t rows = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+    void* vp = nullptr;
+    if (v.has_value() && v->defined()) {
+        check_f16_cuda(*v, "v");
+        TORCH_CHECK(v->sizes() == k.sizes(), "v must be shaped like k");
+        vp = v->data_ptr();
+    }
+    TORCH_CHECK(qkv.scalar_type() == torch::kHalf && qkv.dim() == 2 && qkv.size(0) == rows &&
+                    qkv.size(1) == (Hq + 2 * Hkv) * D && qkv.stride(1) == 1,
+                "qkv must be float16 [rows, (Hq + 2 Hkv) D] with contiguous rows");
+    TORCH_CHECK(q_weight.dim() == 1 && q_weight.size(0) == D && k_weight.dim() == 1 && k_weight.size(0) == D,
+                "q_weight and k_weight must be [D]");
+    TORCH_CHECK(pos.is_cuda() && pos.scalar_type() == torch::kInt64 && pos.numel() == rows && pos.is_contiguous(),
+                "pos must be a contiguous CUDA int64 [rows] tensor");
+    TORCH_CHECK(cos_table.is_cuda() && cos_table.scalar_type() == torch::kFloat32 && cos_table.is_contiguous() &&
+                    cos_table.dim() == 2 && cos_table.size(1) * 2 == D && sin_table.is_cuda() &&
+                    sin_table.sizes() == cos_table.sizes() && sin_table.is_contiguous() &&
+                    sin_table.scalar_type() == torch::kFloat32,
+                "cos / sin tables must be contiguous CUDA float32 [positions, D / 2]");
+    check_status(mg_qk_norm_rope_f16(qkv.data_ptr(), rows == 1 ? qkv.size(1) : qkv.stride(0), q_weight.data_ptr(),
+                                     k_weight.data_ptr(), pos.data_ptr<int64_t>(), cos_table.data_ptr<float>(),
+                                     sin_table.data_ptr<float>(), cos_table.size(0), static_cast<float>(eps),
+                                     q.data_ptr(), k.data_ptr(), vp, rows, static_cast<int32_t>(Hq),
+                                     static_cast<int32_t>(Hkv), static_cast<int32_t>(D), status_ptr(status),
+                                     cur_stream()),
+                 "qk_norm_rope");
 }
 
 torch::Tensor silu_mul(torch::Tensor gu) {
@@ -710,6 +942,29 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("rope_qkv", &rope_qkv, "Split q | k | v, rotary embedding of q and k at per-row positions",
           pybind11::arg("qkv"), pybind11::arg("pos"), pybind11::arg("cos_table"), pybind11::arg("sin_table"),
           pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"));
+    m.def("qk_norm_rope", &qk_norm_rope,
+          "RMS norm of every q and k head and its rotary embedding at per-row positions, in one pass over a q|k|v "
+          "projection (v copied when given)",
+          pybind11::arg("qkv"), pybind11::arg("q_weight"), pybind11::arg("k_weight"), pybind11::arg("pos"),
+          pybind11::arg("cos"), pybind11::arg("sin"), pybind11::arg("eps"), pybind11::arg("q"), pybind11::arg("k"),
+          pybind11::arg("v") = pybind11::none(), pybind11::arg("status") = pybind11::none());
+    m.def("tree_plan", &tree_plan, "Work split of a step's drafted-token attention: (plan and workspace, plan bytes)",
+          pybind11::arg("k_pool"), pybind11::arg("block_tables"), pybind11::arg("seq_lens"),
+          pybind11::arg("max_draft"), pybind11::arg("num_q_heads"), pybind11::arg("n_draft") = pybind11::none(),
+          pybind11::arg("status") = pybind11::none());
+    m.def("tree_attention", &tree_attention, "Attention of drafted tokens over one layer of the cache and each other",
+          pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("mask"), pybind11::arg("k_pool"),
+          pybind11::arg("v_pool"), pybind11::arg("k_scales"), pybind11::arg("v_scales"), pybind11::arg("staging_k"),
+          pybind11::arg("staging_v"), pybind11::arg("block_tables"), pybind11::arg("layer"), pybind11::arg("plan"),
+          pybind11::arg("plan_bytes"), pybind11::arg("scale"), pybind11::arg("out"),
+          pybind11::arg("status") = pybind11::none());
+    m.def("fork_workspace_bytes", &fork_workspace_bytes, "Workspace bytes for fork_sequences");
+    m.def("fork_sequences", &fork_sequences, "Make sequences copies of others: shared pages, copied exact rows",
+          pybind11::arg("free_stack"), pybind11::arg("n_free"), pybind11::arg("in_use"), pybind11::arg("k_pool"),
+          pybind11::arg("v_pool"), pybind11::arg("k_scales"), pybind11::arg("v_scales"), pybind11::arg("staging_k"),
+          pybind11::arg("staging_v"), pybind11::arg("block_tables"), pybind11::arg("seq_lens"),
+          pybind11::arg("src_ids"), pybind11::arg("dst_ids"), pybind11::arg("new_lens"), pybind11::arg("workspace"),
+          pybind11::arg("status") = pybind11::none());
     m.def("silu_mul", &silu_mul, "silu(gate) * up of a [.., 2F] gate | up tensor", pybind11::arg("gu"));
     m.def("version", []() { return std::string(mg_version()); });
 }

@@ -49,18 +49,37 @@ __global__ void __launch_bounds__(kPlanThreads) free_sequences_kernel(int32_t* f
     __shared__ int scratch[33];
     __shared__ int s_dup;
     int top = *n_free_p;
+    // One holder of page row[j] lets go (in_use counts the sequences that hold
+    // a page, mg_fork_sequences); 1 when the page goes back to the stack with
+    // this entry.  Of the entries of one round that hold the same page the last
+    // one returns it, as freeing them one after the other would; entries can
+    // only meet on a page that some entry saw with further holders.  Called by
+    // the whole CTA.
     auto free_page = [&](const int32_t* row, int j, bool live, int32_t& page) -> int {
-        if (!live) return 0;
-        page = row[j];
-        if (page < 0 || page >= num_pages) {
-            flag(status, MG_DEV_BAD_PAGE_ID);
-            return 0;
+        int holders = 0;
+        if (live) {
+            page = row[j];
+            if (page < 0 || page >= num_pages) {
+                flag(status, MG_DEV_BAD_PAGE_ID);
+            } else {
+                holders = atomicSub(&in_use[page], 1);
+                if (holders <= 0) {
+                    atomicAdd(&in_use[page], 1);
+                    flag(status, MG_DEV_DOUBLE_FREE);
+                }
+            }
         }
-        if (atomicExch(&in_use[page], 0) != 1) {
-            flag(status, MG_DEV_DOUBLE_FREE);
-            return 0;
-        }
-        return 1;
+        if (!__syncthreads_or(holders > 1)) return holders == 1;
+        const int mark = -static_cast<int>(threadIdx.x) - 1;
+        const bool gone = holders > 0 && atomicAdd(&in_use[page], 0) == 0;
+        __syncthreads();
+        if (gone) atomicMin(&in_use[page], mark);
+        __syncthreads();
+        const bool last = gone && atomicAdd(&in_use[page], 0) == mark;
+        __syncthreads();
+        if (last) atomicExch(&in_use[page], 0);
+        __syncthreads();
+        return last;
     };
     bool sequential = sm_words == 0;
     if (!sequential) {
@@ -112,8 +131,9 @@ __global__ void __launch_bounds__(kPlanThreads) free_sequences_kernel(int32_t* f
             const int total = run;
             for (int t0 = 0; t0 < total; t0 += blockDim.x) {
                 const int t = t0 + threadIdx.x;
-                int ok = 0;
                 int32_t page = -1;
+                const int32_t* row = nullptr;
+                int j = 0;
                 if (t < total) {
                     int lo = 0, hi = num_seqs - 1;  // last entry i with base[i] <= t
                     while (lo < hi) {
@@ -121,9 +141,10 @@ __global__ void __launch_bounds__(kPlanThreads) free_sequences_kernel(int32_t* f
                         if (base[mid] <= t) lo = mid;
                         else hi = mid - 1;
                     }
-                    const int32_t* row = block_tables + static_cast<int64_t>(seq_ids[lo]) * max_blocks;
-                    ok = free_page(row, keep[lo] + (t - base[lo]), true, page);
+                    row = block_tables + static_cast<int64_t>(seq_ids[lo]) * max_blocks;
+                    j = keep[lo] + (t - base[lo]);
                 }
+                const int ok = free_page(row, j, t < total, page);
                 int cnt;
                 const int excl = block_exclusive_scan(ok, scratch, &cnt);
                 if (ok) free_stack[top + excl] = page;
