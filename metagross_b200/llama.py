@@ -9,6 +9,12 @@ torch fp16 ops (cuBLAS GEMMs); the cache side is this package's: every layer
 appends its new K/V (quantized full pages, exact staged tail) and runs the
 fused paged decode attention.  A decode step is captured in one CUDA graph.
 
+``verify`` runs a tree of drafted tokens per sequence through the model in one
+step (attention over the cache and, by the tree's mask, over each other) and
+appends the tokens that greedy decoding would have produced; ``fork`` makes
+sequences copies of others (several samples of one prompt).  A shape with
+``qk_norm`` normalises every q and k head before the rotation.
+
 Weights are random (seeded) unless given: the benchmarked quantity is the
 decode throughput of the architecture, not its text.
 """
@@ -20,6 +26,7 @@ import torch
 import torch.nn.functional as F
 
 from .batched import BatchedPagedKVCache, _get_C
+from .tree import tree_depths, tree_mask
 
 
 @dataclass(frozen=True)
@@ -32,6 +39,7 @@ class LlamaShape:
     ffn: int = 5632
     rope_theta: float = 10000.0
     rms_eps: float = 1e-5
+    qk_norm: bool = False  # RMS norm of every q and k head (weights "<layer>.qn", "<layer>.kn") before the rotation
 
     @property
     def head_dim(self) -> int:
@@ -73,6 +81,9 @@ class LlamaDecoder:
                 weights[f"{i}.wdown"] = rnd(Fd, H)
                 weights[f"{i}.n1"] = torch.ones(H, device=self.device, dtype=dt)
                 weights[f"{i}.n2"] = torch.ones(H, device=self.device, dtype=dt)
+                if shape.qk_norm:
+                    weights[f"{i}.qn"] = 1 + rnd(D, std=0.1)
+                    weights[f"{i}.kn"] = 1 + rnd(D, std=0.1)
         self.w = weights
         inv = 1.0 / (shape.rope_theta ** (torch.arange(0, D, 2, device=self.device, dtype=torch.float32) / D))
         ang = torch.outer(torch.arange(max_len, device=self.device, dtype=torch.float32), inv)
@@ -113,7 +124,10 @@ class LlamaDecoder:
         D = s.head_dim
         qkv = h @ self.w[f"{i}.wqkv"]
         q, k, v = qkv.split([s.heads * D, s.kv_heads * D, s.kv_heads * D], dim=-1)
-        return (q.unflatten(-1, (s.heads, D)), k.unflatten(-1, (s.kv_heads, D)), v.unflatten(-1, (s.kv_heads, D)))
+        q, k, v = q.unflatten(-1, (s.heads, D)), k.unflatten(-1, (s.kv_heads, D)), v.unflatten(-1, (s.kv_heads, D))
+        if s.qk_norm:
+            q, k = self._rms(q, self.w[f"{i}.qn"]), self._rms(k, self.w[f"{i}.kn"])
+        return q, k, v
 
     def _mlp(self, i, x):
         h = self._rms(x, self.w[f"{i}.n2"])
@@ -134,6 +148,14 @@ class LlamaDecoder:
         x.addmm_(C.silu_mul(gu), self.w[f"{i}.wdown"])
         return x
 
+    def _split(self, i, qkv, pos, q, k, v):
+        """q | k | v of the projection's rows, q and k (normalised and) rotated at positions pos."""
+        C, w = _get_C(), self.w
+        if self.s.qk_norm:
+            C.qk_norm_rope(qkv, w[f"{i}.qn"], w[f"{i}.kn"], pos, self.cos, self.sin, self.s.rms_eps, q, k, v)
+        else:
+            C.rope_qkv(qkv, pos, self.cos, self.sin, q, k, v)
+
     # ---------------------------------------------------------------- prefill
     @torch.no_grad()
     def prefill(self, prompt: torch.Tensor) -> torch.Tensor:
@@ -141,7 +163,7 @@ class LlamaDecoder:
         B, T = prompt.shape
         if B != self.batch or T + 1 > self.max_len:
             raise ValueError("prompt must be [batch, T] with T < max_len")
-        s, c, C = self.s, self.cache, _get_C()
+        s, c = self.s, self.cache
         D = s.head_dim
         x = self.w["embed"][prompt.to(self.device)].reshape(B * T, s.hidden)
         pos = torch.arange(T, device=self.device).repeat(B)
@@ -151,7 +173,7 @@ class LlamaDecoder:
         c.begin_step(T)
         for i in range(s.layers):
             qkv = self._norm(x, self.w[f"{i}.n1"]) @ self.w[f"{i}.wqkv"]
-            C.rope_qkv(qkv, pos, self.cos, self.sin, q, k, v)  # k and v also feed the prompt's own attention
+            self._split(i, qkv, pos, q, k, v)  # k and v also feed the prompt's own attention
             c.append(i, k.view(B, T, s.kv_heads, D), v.view(B, T, s.kv_heads, D))
             o = F.scaled_dot_product_attention(q.view(B, T, s.heads, D).transpose(1, 2),
                                                k.view(B, T, s.kv_heads, D).transpose(1, 2),
@@ -171,15 +193,15 @@ class LlamaDecoder:
         Per layer: RMSNorm, the qkv GEMM, the KV append with the rotary
         embedding fused in (it also writes the rotated q), paged attention, the
         o-projection GEMM accumulated into x, then the MLP."""
-        c, C = self.cache, _get_C()
+        c = self.cache
         x = self.w["embed"][self.ids]
         c.begin_step(1, plan=True)
         for i in range(self.s.layers):
             qkv = self._norm(x, self.w[f"{i}.n1"]) @ self.w[f"{i}.wqkv"]
-            if self.fused_rope:
+            if self.fused_rope and not self.s.qk_norm:
                 c.append_rope(i, qkv, self.s.heads, self.cos, self.sin, self.qb)
             else:
-                C.rope_qkv(qkv, self.pos, self.cos, self.sin, self.qb, self.kb, self.vb)
+                self._split(i, qkv, self.pos, self.qb, self.kb, self.vb)
                 c.append(i, self.kb, self.vb)
             o = c.attend(i, self.qb, out=self.attn_out, max_context=c.max_blocks * c.page_size)
             x.addmm_(o.view(self.batch, -1), self.w[f"{i}.wo"])
@@ -189,6 +211,67 @@ class LlamaDecoder:
             self.logits.copy_(logits)
         self.ids.copy_(logits.argmax(-1))
         self.pos += 1
+
+    # ------------------------------------------------- drafted and forked sequences
+    @torch.no_grad()
+    def verify(self, drafts: torch.Tensor, parents) -> tuple[torch.Tensor, torch.Tensor]:
+        """One step that checks a tree of drafted tokens per sequence.
+
+        drafts [B, T]: column 0 is the pending token (``ids``), the others are guesses of what
+        follows; parents [T] or [B, T]: each token's parent, below its own index (-1 for column
+        0).  Every token runs through the model at its depth's position.  A guess is accepted
+        if its parent is and the model's greedy token after the parent is the guess; the
+        longest accepted path is appended to the cache and ``ids`` becomes the model's token
+        after it.  Returns (tokens [B, T] of the path, in order, and their counts [B], >= 1)."""
+        s, c, dev = self.s, self.cache, self.device
+        B, T = drafts.shape
+        if B != self.batch or T < 1:
+            raise ValueError(f"drafts must be [{self.batch}, at least 1]")
+        drafts = drafts.to(dev)
+        mask = tree_mask(parents).to(dev).expand(B, T, T)
+        parents = torch.as_tensor(parents).long().to(dev).expand(B, T)
+        depth = tree_depths(mask)
+        hq, hkv, D, L = s.heads, s.kv_heads, s.head_dim, s.layers
+        pos = (self.pos[:, None] + depth).reshape(-1)
+        x = self.w["embed"][drafts].reshape(B * T, s.hidden)
+        q = torch.empty(B * T, hq, D, dtype=x.dtype, device=dev)
+        k = torch.empty(L, B * T, hkv, D, dtype=x.dtype, device=dev)
+        v = torch.empty_like(k)
+        plan = c.plan_tree(T, hq)
+        for i in range(L):
+            qkv = self._norm(x, self.w[f"{i}.n1"]) @ self.w[f"{i}.wqkv"]
+            self._split(i, qkv, pos, q, k[i], v[i])
+            o = c.attend_tree(i, q.view(B, T, hq, D), k[i].view(B, T, hkv, D), v[i].view(B, T, hkv, D), mask=mask,
+                              plan=plan)
+            x.addmm_(o.view(B * T, hq * D), self.w[f"{i}.wo"])
+            self._ffn(i, x)
+        nxt = (self._norm(x, self.w["norm"]) @ self.w["lm_head"]).argmax(-1).view(B, T)
+        # a token is accepted when it and all its ancestors are what their parents predict
+        right = (drafts == nxt.gather(1, parents.clamp(min=0))) | (parents < 0)
+        accepted = (right[:, None] | ~mask).all(-1)
+        best = torch.where(accepted, depth, -1).argmax(1, keepdim=True)  # the first of the deepest
+        count = depth.gather(1, best) + 1
+        # the ancestors of `best`, in index order, which is depth order
+        on_path = mask.gather(1, best[..., None].expand(B, 1, T))[:, 0]
+        path = torch.where(on_path, 0, T) + torch.arange(T, device=dev)
+        path = path.sort(1).values.remainder(T)
+        n = count[:, 0].to(torch.int32)
+        rows = (path + T * torch.arange(B, device=dev)[:, None]).reshape(-1)
+        k, v = (y.index_select(1, rows).view(L, B, T, hkv, D) for y in (k, v))
+        c.begin_step(n)
+        for i in range(L):
+            c.append(i, k[i], v[i])
+        self.ids.copy_(nxt.gather(1, best)[:, 0])
+        self.pos += n
+        return drafts.gather(1, path), n
+
+    def fork(self, src, dst) -> None:
+        """Sequences dst become copies of sequences src: the cache (shared pages, copied exact
+        rows), the position and the pending token."""
+        self.cache.fork(src, dst)
+        src, dst = (torch.as_tensor(x).long().to(self.device) for x in (src, dst))
+        self.ids[dst] = self.ids[src]
+        self.pos[dst] = self.pos[src]
 
     def capture(self) -> None:
         """Capture the decode step in a CUDA graph (after prefill)."""
@@ -206,7 +289,7 @@ class LlamaDecoder:
         torch.cuda.current_stream(self.device).wait_stream(st)
         self.ids.copy_(saved[0])
         self.pos.copy_(saved[1])
-        c._plan_ok = False
+        c.invalidate_plan()
 
     @torch.no_grad()
     def decode(self, n: int) -> torch.Tensor:
@@ -221,7 +304,7 @@ class LlamaDecoder:
                 c._ensure_n_new(1)
                 self.graph.replay()
                 c._max_len = min(c._max_len + 1, c.max_blocks * c.page_size + c.page_size - 1)
-                c._plan_ok = False
+                c.invalidate_plan()
             else:
                 self._step()
         return out
