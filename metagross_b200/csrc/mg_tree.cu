@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kTreePlanThreads) tree_plan_kernel(TreePlanPar
             n = t = 0;
         }
         const int mt = cdiv(t * a.G, a.geo.BM);
-        const int U = t == 0 ? 0 : cdiv(n, kTreeTile) + cdiv(t, kTreeTile);
+        const int U = t == 0 ? 0 : cdiv(n, a.geo.tile) + cdiv(t, a.geo.tile);
         int4* rec = reinterpret_cast<int4*>(seqs + static_cast<int64_t>(b) * 8);
         rec[0] = make_int4(t, 0, 0, n);
         rec[1] = make_int4(0, mt, U, 0);
@@ -217,6 +217,9 @@ mg_status check_tree(const mg_cache_layout* L, int64_t batch, int64_t T, int64_t
     MG_REQUIRE(Hq >= 1 && Hq % L->num_kv_heads == 0, "num_q_heads=%lld must be a positive multiple of num_kv_heads=%d",
                (long long)Hq, L->num_kv_heads);
     MG_REQUIRE(T * Hq < (1ll << 31), "max_draft * num_q_heads too large");
+    MG_REQUIRE((L->max_blocks + 1ll) * L->page_size < (1ll << 26),
+               "drafted-token attention supports contexts below 2^26 tokens, got max_blocks=%d pages of %d",
+               L->max_blocks, L->page_size);
     const TreeGeom g = tree_geometry(*L, batch, T, Hq);
     MG_REQUIRE(g.max_items * L->num_kv_heads < (1ll << 31), "too many work items for one launch");
     return MG_OK;
@@ -235,12 +238,24 @@ TreeGeom tree_geometry(const mg_cache_layout& L, int64_t batch, int64_t T, int64
     TreeGeom g;
     const int64_t rows = T * (Hq / L.num_kv_heads);
     int occ;
-    if (L.head_dim == 64 && rows > 16) {
-        g.BM = 32;
-        occ = rows_ctas_per_sm<64, 2>();
+    // Above 48 rows the tensor-core tile kernel, whose time hardly depends on the
+    // rows (one B200, us per call): head_dim 64, 64 sequences of 1000 tokens, 4 kv
+    // heads, INT8: 32 rows 34 (row kernel) / 61 (tile kernel), 64 rows 65 / 67, 128
+    // rows 93 / 85; 200 sequences of 3000, INT4: 32 rows 178 / 221, 40 rows 267 /
+    // 226, 128 rows 548 / 254; head_dim 128, 12 sequences of 3000, INT8: 48 rows 65 /
+    // 76, 64 rows 113 / 77, 128 rows 190 / 86.
+    g.tiles = rows > 48;
+    if (g.tiles) {
+        g.tile = kTilesKeys;
+        // equal row tiles of at most 128, in whole warps
+        const int64_t mt = rows > 128 ? (rows + 127) / 128 : 1;
+        g.BM = static_cast<int>(((rows + mt - 1) / mt + 31) / 32 * 32);
+        occ = 1;
     } else {
-        g.BM = 16;
-        occ = L.head_dim == 64 ? rows_ctas_per_sm<64, 1>() : rows_ctas_per_sm<128, 1>();
+        g.tile = kTreeTile;
+        g.BM = L.head_dim == 64 && rows > 16 ? 32 : 16;
+        occ = L.head_dim == 128 ? rows_ctas_per_sm<128, 1>()
+                                : (g.BM == 32 ? rows_ctas_per_sm<64, 2>() : rows_ctas_per_sm<64, 1>());
     }
     g.mt_max = static_cast<int>((rows + g.BM - 1) / g.BM);
     g.slots = sm_count() * occ;
@@ -348,6 +363,7 @@ extern "C" mg_status mg_tree_attention(const mg_cache_layout* L, const mg_layer_
     p.block_tables = block_tables;
     p.max_blocks = L->max_blocks;
     p.P = L->page_size;
+    p.div_p = FastDiv(static_cast<uint32_t>(L->page_size));
     p.Hkv = L->num_kv_heads;
     p.G = d->num_q_heads / L->num_kv_heads;
     p.scale_th = L->scale_layout == MG_SCALE_TOKEN_HEAD;
@@ -362,6 +378,7 @@ extern "C" mg_status mg_tree_attention(const mg_cache_layout* L, const mg_layer_
     p.mask_sb = d->mask_stride;
     p.T = d->max_draft;
     p.batch = batch;
+    p.BM = g.BM;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.out = static_cast<__half*>(out);
     p.plan = static_cast<const int32_t*>(plan);
@@ -371,7 +388,10 @@ extern "C" mg_status mg_tree_attention(const mg_cache_layout* L, const mg_layer_
     p.status = dev_status;
     cudaStream_t s = as_stream(stream);
     const bool i4 = L->kv_dtype == MG_KV_INT4;
-    if (L->head_dim == 64) i4 ? launch_tree_rows<true, 64>(p, g, s) : launch_tree_rows<false, 64>(p, g, s);
+    if (g.tiles) {
+        if (L->head_dim == 64) i4 ? launch_tree_tiles<true, 64>(p, g, s) : launch_tree_tiles<false, 64>(p, g, s);
+        else i4 ? launch_tree_tiles<true, 128>(p, g, s) : launch_tree_tiles<false, 128>(p, g, s);
+    } else if (L->head_dim == 64) i4 ? launch_tree_rows<true, 64>(p, g, s) : launch_tree_rows<false, 64>(p, g, s);
     else i4 ? launch_tree_rows<true, 128>(p, g, s) : launch_tree_rows<false, 128>(p, g, s);
     st = check_launch("tree_rows_kernel");
     if (st != MG_OK) return st;

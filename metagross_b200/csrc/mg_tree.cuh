@@ -4,8 +4,8 @@
 // Notation: G = Hq / Hkv query heads share a kv head; the R = t * G query rows
 // of one (sequence, kv head) -- t drafted tokens, row r = token r / G, head
 // r % G of the group -- all read the same keys, so they are computed together
-// in row tiles of BM.  Keys are counted in tiles of kTreeTile tokens: the
-// cached context's tiles (pages, then the staged tail) first, then the
+// in row tiles of BM.  Keys are counted in tiles (64 or 128 tokens, by kernel):
+// the cached context's tiles (pages, then the staged tail) first, then the
 // drafted tokens'.
 #pragma once
 
@@ -14,13 +14,16 @@
 
 namespace mg {
 
-constexpr int kTreeTile = 64;       // keys per unit of the plan
+constexpr int kTreeTile = 64;       // keys of a tile of the row kernel
+constexpr int kTilesKeys = 128;     // keys of a tile of the tensor-core tile kernel
 constexpr int kTreeHeader = 16;     // int32 words before the plan's records
 constexpr int kTreeMaxBatch = 65535;
 
 // What the host fixes for one (layout, batch, drafted tokens, q heads): the
 // row tile, how many CTAs run at once, and the bounds on the work items.
 struct TreeGeom {
+    bool tiles;        // the tensor-core tile kernel, else the row kernel
+    int tile;          // keys per unit of the plan
     int BM;            // query rows per work item
     int mt_max;        // row tiles of a sequence that drafts T tokens
     int slots;         // CTAs resident on the GPU at once
@@ -55,6 +58,7 @@ struct TreeParams {
     const int32_t* block_tables;
     int32_t max_blocks;
     int32_t P;
+    FastDiv div_p;  // by P, exact below 2^26 tokens
     int32_t Hkv;
     int32_t G;
     int32_t scale_th;  // scales [N, P, Hkv] instead of [N]
@@ -69,6 +73,7 @@ struct TreeParams {
     int64_t mask_sb;
     int32_t T;
     int32_t batch;
+    int32_t BM;  // query rows per work item
     float scale_log2;  // attention scale * log2(e)
     __half* out;       // [batch, T, Hq, D]
     const int32_t* plan;
@@ -87,16 +92,19 @@ __device__ __forceinline__ bool tree_plan_matches(const TreeParams& p, int BM) {
 // device helpers shared by the kernels
 // ---------------------------------------------------------------------------
 
-// A V scale s as s = mant * 2^e with e in [-20, 5]: the codes times 2^e are
-// exact in fp16 over that whole range (|code| <= 127, and |code| * 2^e never
-// exceeds the page's absmax), and mant, which goes into the fp32
-// probabilities, is in [1, 2) unless s itself is outside 2^-20 .. 2^6.  So a
-// page of very small or very large values loses nothing to fp16's exponent
-// range, which the plain product probability * s would.
+// A V scale s as s = mant * 2^e with e in [-20, 13]: the codes times 2^e are
+// exact in fp16 over that whole range (|code| * 2^e never exceeds the page's
+// absmax, which fp16 holds), and mant, which goes into the fp32 probabilities, is
+// below 2, and at least 1 unless s is below 2^-20.  So a page of very small or
+// very large values loses nothing to fp16's exponent range, which the plain
+// product probability * s would.
 __device__ __forceinline__ int scale_exponent(float s) {
     const int e = static_cast<int>((__float_as_uint(s) >> 23) & 255u) - 127;
-    return e < -20 ? -20 : (e > 5 ? 5 : e);
+    return e < -20 ? -20 : (e > 13 ? 13 : e);
 }
+// The part of 2^e that the conversion's one fp16 FMA can hold: its offset of
+// 1152 * 2^e has to fit as well.  Scales of 64 and more need a second step.
+__device__ __forceinline__ int fma_exponent(int e) { return e > 5 ? 5 : e; }
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ uint32_t half_bits(float x) {
     return static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x)));
@@ -150,6 +158,9 @@ __host__ __device__ constexpr int rows_ctas_per_sm() {
 // host: kernel launchers (one translation unit per pool format and head_dim)
 template <bool KV4, int D>
 void launch_tree_rows(const TreeParams& p, const TreeGeom& g, cudaStream_t stream);
+
+template <bool KV4, int D>
+void launch_tree_tiles(const TreeParams& p, const TreeGeom& g, cudaStream_t stream);
 
 TreeGeom tree_geometry(const mg_cache_layout& L, int64_t batch, int64_t T, int64_t Hq);
 

@@ -70,7 +70,8 @@ __device__ __forceinline__ void half_pair(const uint32_t* x, int s, uint32_t& b0
     b1 = prmt(lo, hi, 0x7632);
 }
 
-// fp16 multiplier and offset that turn an exponent-inserted code into code * 2^e
+// fp16 multiplier and offset that turn an exponent-inserted code into code * 2^e,
+// e up to 5 (see fma_exponent; groups with larger scales take the general path)
 struct VScale {
     uint32_t mul, bias;       // INT8, or the low nibbles
     uint32_t mul_hi, bias_hi;  // the high nibbles (inserted as 16 * code)
@@ -299,7 +300,9 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
     };
     auto group_page = [&](int tok0) { return page_of(UNI ? tok0 : tok0 + (lane & 15)); };
     const int wt = 16 * warp;
-    int jp = j0;  // first tile after the paged groups of this warp
+    int jp = j0;           // first tile after the paged groups of this warp
+    bool some_big = false;  // a group had a V scale of 64 or more and is left for later
+    auto big = [](float v) { return fma_exponent(scale_exponent(v)) != scale_exponent(v); };
     {
         const int lim = whole - wt - 16;
         const int jend = lim < 0 ? j0 : min(j1, lim / kTreeTile + 1);
@@ -313,6 +316,12 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 if (j + 1 < jend) {
                     load_raw((j + 1) * kTreeTile + wt, page, nxt);
                     if (j + 2 < jend) page = group_page((j + 2) * kTreeTile + wt);
+                }
+                bool over = big(cur.vs[0]);
+                if constexpr (!UNI) over |= big(cur.vs[1]) | big(cur.vs[2]) | big(cur.vs[3]);
+                if (__any_sync(0xffffffffu, over)) {
+                    some_big = true;
+                    continue;
                 }
                 float ks[4], vm[4];
                 VScale vsc[2];
@@ -340,7 +349,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
 
     // ---- groups with staged rows, and the drafted tokens: fragments of halves
     bool bad = false;
-    uint32_t kh[2][D / 8], vh[4][D / 16];
+    uint32_t kh[2][D / 8] = {}, vh[4][D / 16] = {};
     auto half_groups = [&](const float (&ks)[4], const float (&vm)[4], auto&& seen) {
         attend([&](int nt, int s, uint32_t& b0, uint32_t& b1) { half_pair<KV4>(kh[nt], s, b0, b1); },
                [&](int jj, uint32_t& b0, uint32_t& b1) {
@@ -364,9 +373,13 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 x[i] = finite_or_zero2(x[i]);
             }
     };
-    for (int j = max(jp, j0); j < min(j1, nct); ++j) {
+    for (int j = some_big ? j0 : jp; j < min(j1, nct); ++j) {
         const int tok0 = j * kTreeTile + wt;
         if (tok0 >= n) break;
+        if (j < jp) {  // of the paged groups, those left for later
+            const int key = tok0 + (lane & 15);
+            if (!__any_sync(0xffffffffu, big(scale_at(p.v_scales, page_of(key), key % p.P)))) continue;
+        }
         clear_half();
         float ks[4], vm[4];
         // a code as a half: its integer value; K's scale goes into the score,
