@@ -17,6 +17,8 @@
 // the instructions.
 #pragma once
 
+#include <type_traits>
+
 #include "mg_tree.cuh"
 
 namespace mg {
@@ -150,7 +152,9 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
     // one group of 16 keys: kfrag(nt, s) and vfrag(j) give the fragments, ks
     // the score factor and vm the probability factor of this lane's keys
     // (2c, 2c+1, 2c+8, 2c+9), seen(rt, u, i) whether row and key meet
-    auto attend = [&](auto&& kfrag, auto&& vfrag, const float (&ks)[4], const float (&vm)[4], auto&& seen) {
+    // (uni: the four are the same, ks is positive and every key is seen)
+    auto attend = [&](auto&& kfrag, auto&& vfrag, const float (&ks)[4], const float (&vm)[4], auto&& seen, auto uni) {
+        constexpr bool kUni = decltype(uni)::value;
         float s[RT][2][4];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -168,6 +172,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 for (int rt = 0; rt < RT; ++rt) mma_16816(s[rt][nt], qf[rt][st], b0, b1);
             }
         uint32_t pf[RT][4];
+        const float lvm = kUni ? __log2f(vm[0]) : 0.0f, ivm = kUni ? __frcp_rn(vm[0]) : 1.0f;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float mx[2] = {-INFINITY, -INFINITY};
@@ -176,9 +181,10 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = nt * 2 + (i & 1), u = i >> 1;
-                    s[rt][nt][i] = seen(rt, u, key) ? s[rt][nt][i] * ks[key] : -INFINITY;
+                    if constexpr (!kUni) s[rt][nt][i] = seen(rt, u, key) ? s[rt][nt][i] * ks[key] : -INFINITY;
                     mx[u] = fmaxf(mx[u], s[rt][nt][i]);
                 }
+            if constexpr (kUni) mx[0] *= ks[0], mx[1] *= ks[0];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
@@ -204,13 +210,27 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const float ref = m[rt][u] == -INFINITY ? 0.0f : m[rt][u];
+                if constexpr (kUni) {
+                    // the V scale's mantissa goes into the exponent, and out of the sum again
+                    const float off = lvm - ref;
+                    float sum = 0.0f;
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const float p0 = ex2(s[rt][nt][2 * u] - ref), p1 = ex2(s[rt][nt][2 * u + 1] - ref);
-                    l[rt][u] += p0 + p1;
-                    // probabilities go to fp16 for the product with V (half a
-                    // unit in 2^11 each); their sum stays in fp32
-                    pf[rt][nt * 2 + u] = pack_half2(p0 * vm[nt * 2], p1 * vm[nt * 2 + 1]);
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const float p0 = ex2(fmaf(s[rt][nt][2 * u], ks[0], off));
+                        const float p1 = ex2(fmaf(s[rt][nt][2 * u + 1], ks[0], off));
+                        sum += p0 + p1;
+                        pf[rt][nt * 2 + u] = pack_half2(p0, p1);
+                    }
+                    l[rt][u] = fmaf(sum, ivm, l[rt][u]);
+                } else {
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const float p0 = ex2(s[rt][nt][2 * u] - ref), p1 = ex2(s[rt][nt][2 * u + 1] - ref);
+                        l[rt][u] += p0 + p1;
+                        // probabilities go to fp16 for the product with V (half a
+                        // unit in 2^11 each); their sum stays in fp32
+                        pf[rt][nt * 2 + u] = pack_half2(p0 * vm[nt * 2], p1 * vm[nt * 2 + 1]);
+                    }
                 }
             }
         }
@@ -227,13 +247,14 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
     const int nct = (n + kTreeTile - 1) / kTreeTile;
     const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.max_blocks;
     auto page_of = [&](int token) -> int32_t {
-        const int32_t pg = bt[token / p.P];
+        const int32_t pg = bt[p.div_p.div(token)];
         if (pg < 0 || pg >= p.num_pages) {
             flag(p.status, MG_DEV_BAD_PAGE_ID);
             return 0;
         }
         return pg;
     };
+    auto slot_of = [&](int token) { return token - static_cast<int>(p.div_p.div(token)) * p.P; };
     auto scale_at = [&](const float* scales, int32_t page, int slot) {
         return p.scale_th ? scales[(static_cast<int64_t>(page) * p.P + slot) * p.Hkv + h] : scales[page];
     };
@@ -267,17 +288,24 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
         uint32_t k[2][F::KW], v[4][F::VW];
         float ks[UNI ? 1 : 4], vs[UNI ? 1 : 4];
     };
+    const int step = p.Hkv * F::kRowBytes;  // bytes from one token to the next
+    const int64_t page_bytes = static_cast<int64_t>(p.P) * step;
+    const uint8_t* k_lane = p.k_pool + static_cast<int64_t>(h) * F::kRowBytes + g * step + c * (F::KW * 4);
+    const uint8_t* v_lane = p.v_pool + static_cast<int64_t>(h) * F::kRowBytes + 2 * c * step + g * (F::VW * 4);
     auto load_raw = [&](int tok0, int32_t page, Raw& r) {
         // page: of the whole group (UNI), else of key lane & 15 of the group
         if constexpr (UNI) {
-            const int slot = tok0 % p.P;
-            const int64_t step = static_cast<int64_t>(p.Hkv) * F::kRowBytes;
-            const uint8_t* kb = row_at(p.k_pool, page, slot) + c * (F::KW * 4);
-            const uint8_t* vb = row_at(p.v_pool, page, slot) + g * (F::VW * 4);
-            ldg_words(r.k[0], kb + g * step);
-            ldg_words(r.k[1], kb + (g + 8) * step);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ldg_words(r.v[i], vb + (2 * c + (i & 1) + 8 * (i >> 1)) * step);
+            const int slot = slot_of(tok0);
+            // one wide multiplication per group; everything else is this lane's own
+            const int64_t at = page * page_bytes + slot * step;
+            const uint8_t* kb = k_lane + at;
+            const uint8_t* vb = v_lane + at;
+            ldg_words(r.k[0], kb);
+            ldg_words(r.k[1], kb + 8 * step);
+            ldg_words(r.v[0], vb);
+            ldg_words(r.v[1], vb + step);
+            ldg_words(r.v[2], vb + 8 * step);
+            ldg_words(r.v[3], vb + 9 * step);
             r.ks[0] = p.k_scales[page];
             r.vs[0] = p.v_scales[page];
         } else {
@@ -285,13 +313,13 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
             for (int i = 0; i < 2; ++i) {
                 const int key = g + 8 * i;
                 const int32_t pg = __shfl_sync(0xffffffffu, page, key);
-                ldg_words(r.k[i], row_at(p.k_pool, pg, (tok0 + key) % p.P) + c * (F::KW * 4));
+                ldg_words(r.k[i], row_at(p.k_pool, pg, slot_of(tok0 + key)) + c * (F::KW * 4));
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = 2 * c + (i & 1) + 8 * (i >> 1);
                 const int32_t pg = __shfl_sync(0xffffffffu, page, key);
-                const int slot = (tok0 + key) % p.P;
+                const int slot = slot_of(tok0 + key);
                 ldg_words(r.v[i], row_at(p.v_pool, pg, slot) + g * (F::VW * 4));
                 r.ks[i] = scale_at(p.k_scales, pg, slot);
                 r.vs[i] = scale_at(p.v_scales, pg, slot);
@@ -302,7 +330,8 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
     const int wt = 16 * warp;
     int jp = j0;           // first tile after the paged groups of this warp
     bool some_big = false;  // a group had a V scale of 64 or more and is left for later
-    auto big = [](float v) { return fma_exponent(scale_exponent(v)) != scale_exponent(v); };
+    // (or one below 2^-60, whose mantissa has no useful reciprocal)
+    auto big = [](float v) { return v >= 64.0f || v < 0x1p-60f; };
     {
         const int lim = whole - wt - 16;
         const int jend = lim < 0 ? j0 : min(j1, lim / kTreeTile + 1);
@@ -341,7 +370,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                            b0 = code_v(cur.v[0][w], cur.v[1][w], e, vsc[0]);
                            b1 = code_v(cur.v[2][w], cur.v[3][w], e, vsc[1]);
                        },
-                       ks, vm, [](int, int, int) { return true; });
+                       ks, vm, [](int, int, int) { return true; }, std::integral_constant<bool, UNI>{});
             }
             jp = jend;
         }
@@ -357,7 +386,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                    b0 = prmt(vh[0][jj >> 1], vh[1][jj >> 1], sel);
                    b1 = prmt(vh[2][jj >> 1], vh[3][jj >> 1], sel);
                },
-               ks, vm, seen);
+               ks, vm, seen, std::false_type{});
     };
     auto clear_half = [&]() {
 #pragma unroll
@@ -378,7 +407,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
         if (tok0 >= n) break;
         if (j < jp) {  // of the paged groups, those left for later
             const int key = tok0 + (lane & 15);
-            if (!__any_sync(0xffffffffu, big(scale_at(p.v_scales, page_of(key), key % p.P)))) continue;
+            if (!__any_sync(0xffffffffu, big(scale_at(p.v_scales, page_of(key), slot_of(key))))) continue;
         }
         clear_half();
         float ks[4], vm[4];
@@ -402,7 +431,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
             const int tk = tok0 + g + 8 * i;
             if (tk < whole) {
                 uint32_t w[F::KW];
-                ldg_words(w, row_at(p.k_pool, page_of(tk), tk % p.P) + c * (F::KW * 4));
+                ldg_words(w, row_at(p.k_pool, page_of(tk), slot_of(tk)) + c * (F::KW * 4));
 #pragma unroll
                 for (int e = 0; e < D / 8; ++e) kh[i][e] = half_code(w, e);
             } else if (tk < n) {
@@ -417,13 +446,13 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
             vm[i] = 1.0f;
             if (tk < whole) {
                 const int32_t pg = page_of(tk);
-                const float vs = scale_at(p.v_scales, pg, tk % p.P);
-                ks[i] = scale_at(p.k_scales, pg, tk % p.P) * p.scale_log2;
+                const float vs = scale_at(p.v_scales, pg, slot_of(tk));
+                ks[i] = scale_at(p.k_scales, pg, slot_of(tk)) * p.scale_log2;
                 const int e2 = scale_exponent(vs);
                 vm[i] = vs * pow2f(-e2);
                 const uint32_t f = half_bits(pow2f(e2)) * 0x10001u;
                 uint32_t w[F::VW];
-                ldg_words(w, row_at(p.v_pool, pg, tk % p.P) + g * (F::VW * 4));
+                ldg_words(w, row_at(p.v_pool, pg, slot_of(tk)) + g * (F::VW * 4));
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e) vh[i][e] = hfma2_u32(half_code(w, e), f, 0u);
             } else if (tk < n) {
