@@ -319,7 +319,8 @@ class BatchedPagedKVCache:
         rows after them are copied, or dequantized where lens cuts a committed page.  What dst
         held is released first.  src, dst, lens: lists or int32 tensors; a target may not be a
         source or appear twice (device tensors: such pairs are skipped and ``check`` raises)."""
-        if not any(isinstance(x, torch.Tensor) and x.is_cuda for x in (src, dst)):
+        on_device = isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and src.is_cuda and dst.is_cuda
+        if not on_device:
             s, d = (torch.as_tensor(x).flatten().tolist() for x in (src, dst))
             if len(s) != len(d):
                 raise ValueError("src and dst must have the same length")
@@ -327,9 +328,9 @@ class BatchedPagedKVCache:
                 raise ValueError(f"sequence ids must be in [0, {self.batch})")
             if len(set(d)) != len(d) or set(d) & set(s):
                 raise ValueError("a target may not be a source or appear twice")
-        ids = [torch.as_tensor(x, dtype=torch.int32).to(self.device).contiguous() for x in (src, dst)]
+        ids = [torch.as_tensor(x, dtype=torch.int32, device=self.device).contiguous() for x in (src, dst)]
         if lens is not None:
-            lens = torch.as_tensor(lens, dtype=torch.int32).to(self.device).contiguous()
+            lens = torch.as_tensor(lens, dtype=torch.int32, device=self.device).contiguous()
         C = _get_C()
         need = C.fork_workspace_bytes(ids[0].numel()) // 4
         if need > self._fork_ws.numel():

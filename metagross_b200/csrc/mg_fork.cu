@@ -196,11 +196,19 @@ __global__ void __launch_bounds__(kForkThreads) fork_share_kernel(ForkParams p) 
         const uint4* vs = reinterpret_cast<const uint4*>(static_cast<const ST*>(p.staging_v) + off + s * pe);
         uint4* kd = reinterpret_cast<uint4*>(static_cast<ST*>(p.staging_k) + off + d * pe);
         uint4* vd = reinterpret_cast<uint4*>(static_cast<ST*>(p.staging_v) + off + d * pe);
-#pragma unroll 4
-        for (int e = threadIdx.x; e < n8 * kWords; e += kForkThreads) {
-            const uint4 a = ks[e], b = vs[e];
-            kd[e] = a;
-            vd[e] = b;
+        constexpr int kBatch = 4;
+        for (int e0 = threadIdx.x; e0 < n8 * kWords; e0 += kForkThreads * kBatch) {
+            uint4 a[kBatch], b[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int e = e0 + u * kForkThreads;
+                if (e < n8 * kWords) a[u] = ks[e], b[u] = vs[e];
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int e = e0 + u * kForkThreads;
+                if (e < n8 * kWords) kd[e] = a[u], vd[e] = b[u];
+            }
         }
         return;
     }
@@ -210,40 +218,57 @@ __global__ void __launch_bounds__(kForkThreads) fork_share_kernel(ForkParams p) 
         if (threadIdx.x == 0) flag(p.status, MG_DEV_BAD_PAGE_ID);
         page = 0;
     }
-    for (int kv = 0; kv < 2; ++kv) {
-        const uint8_t* pool =
-            (kv ? p.v_pool : p.k_pool) + p.pool_layer * layer + static_cast<int64_t>(page) * (INT4 ? pe / 2 : pe);
-        const float* scales = (kv ? p.v_scales : p.k_scales) + p.scale_layer * layer;
-        ST* to = static_cast<ST*>(kv ? p.staging_v : p.staging_k) + p.staging_layer * layer + d * pe;
-        const float page_scale = p.scale_th ? 0.0f : scales[page];
-#pragma unroll 2
-        for (int g = threadIdx.x; g < n8; g += kForkThreads) {
-            const int e = g * 8;
-            // [page][token][head]: one scale per D elements
-            const float sf =
-                p.scale_th ? scales[static_cast<int64_t>(page) * (pe / p.D) + e / p.D] : page_scale;
-            float v[8];
-            if constexpr (INT4) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(pool + e / 2);
+    const int64_t page_at = static_cast<int64_t>(page) * (INT4 ? pe / 2 : pe);
+    const uint8_t* pool[2] = {p.k_pool + p.pool_layer * layer + page_at, p.v_pool + p.pool_layer * layer + page_at};
+    const float* scales[2] = {p.k_scales + p.scale_layer * layer, p.v_scales + p.scale_layer * layer};
+    ST* to[2] = {static_cast<ST*>(p.staging_k) + p.staging_layer * layer + d * pe,
+                 static_cast<ST*>(p.staging_v) + p.staging_layer * layer + d * pe};
+    const float page_scale[2] = {p.scale_th ? 0.0f : scales[0][page], p.scale_th ? 0.0f : scales[1][page]};
+    // K and V of kBatch groups of 8 in flight before the first is stored
+    constexpr int kBatch = 4;
+    for (int g0 = threadIdx.x; g0 < n8; g0 += kForkThreads * kBatch) {
+        uint2 w[kBatch][2];
+        float sf[kBatch][2];
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    v[q] = static_cast<float>(static_cast<int32_t>(w << (28 - 4 * q)) >> 28) * sf;
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(pool + e);
+        for (int u = 0; u < kBatch; ++u)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    v[q] = static_cast<float>(static_cast<int8_t>(w.x >> (8 * q))) * sf;
-                    v[4 + q] = static_cast<float>(static_cast<int8_t>(w.y >> (8 * q))) * sf;
+            for (int kv = 0; kv < 2; ++kv) {
+                const int e = (g0 + u * kForkThreads) * 8;
+                w[u][kv] = make_uint2(0u, 0u);
+                sf[u][kv] = page_scale[kv];
+                if (e >= n8 * 8) continue;
+                if constexpr (INT4) w[u][kv].x = *reinterpret_cast<const uint32_t*>(pool[kv] + e / 2);
+                else w[u][kv] = *reinterpret_cast<const uint2*>(pool[kv] + e);
+                // [page][token][head]: one scale per D elements
+                if (p.scale_th) sf[u][kv] = scales[kv][static_cast<int64_t>(page) * (pe / p.D) + e / p.D];
+            }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                const int e = (g0 + u * kForkThreads) * 8;
+                if (e >= n8 * 8) continue;
+                float v[8];
+                if constexpr (INT4) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        v[q] = static_cast<float>(static_cast<int32_t>(w[u][kv].x << (28 - 4 * q)) >> 28) * sf[u][kv];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        v[q] = static_cast<float>(static_cast<int8_t>(w[u][kv].x >> (8 * q))) * sf[u][kv];
+                        v[4 + q] = static_cast<float>(static_cast<int8_t>(w[u][kv].y >> (8 * q))) * sf[u][kv];
+                    }
+                }
+                if constexpr (sizeof(ST) == 2) {
+                    *reinterpret_cast<uint4*>(to[kv] + e) =
+                        make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]),
+                                   pack_half2(v[6], v[7]));
+                } else {
+                    *reinterpret_cast<float4*>(to[kv] + e) = make_float4(v[0], v[1], v[2], v[3]);
+                    *reinterpret_cast<float4*>(to[kv] + e + 4) = make_float4(v[4], v[5], v[6], v[7]);
                 }
             }
-            if constexpr (sizeof(ST) == 2) {
-                *reinterpret_cast<uint4*>(to + e) = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]),
-                                                               pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
-            } else {
-                *reinterpret_cast<float4*>(to + e) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4*>(to + e + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            }
-        }
     }
 }
 

@@ -7,6 +7,8 @@
 //
 // Bound: each value is read and written once, so HBM for prompts and the
 // launch for a decode step.
+#include <type_traits>
+
 #include "mg_common.cuh"
 
 namespace mg {
@@ -58,10 +60,13 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 // row's cos and sin, 8 of each per lane, serve all its heads: a warp takes a
 // row (or one of `parts` shares of its heads) and keeps them in registers.
 // `parts` is 1 once the rows alone fill the GPU, and splits the row below that.
-template <int LPH>
+// U rounds of heads are in flight.  One B200, 18423 rows of 32 + 8 + 8 heads of 128
+// (453 MB): 98 / 95 / 88 / 91 us with U = 1 / 2 / 3 / 4 (5.2 TB/s, 0.79 of the
+// copy rate); 1024 rows of 32 + 4 heads of 64, a round per warp: 4.5 us with U = 1,
+// 5.7 with 2 (the second round's registers cost resident warps).
+template <int LPH, int U>
 __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(QkNormParams p) {
     constexpr int HPW = 32 / LPH;  // heads a warp takes at once
-    constexpr int U = 2;           // of which two rounds are in flight
     grid_dependency_wait();
     grid_launch_dependents();
     const int lane = threadIdx.x & 31, j = lane % LPH, sub = lane / LPH;
@@ -234,12 +239,17 @@ extern "C" mg_status mg_qk_norm_rope_f16(const void* qkv, int64_t row_stride, co
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    auto go = [&](auto lanes) {
+        constexpr int kLanes = decltype(lanes)::value;
+        if (p.parts == 1) cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<kLanes, 3>, p);
+        else cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<kLanes, 1>, p);
+    };
     if (!vec) cudaLaunchKernelEx(&cfg, qk_norm_rope_any_kernel, p);
-    else if (lph == 1) cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<1>, p);
-    else if (lph == 2) cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<2>, p);
-    else if (lph == 4) cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<4>, p);
-    else if (lph == 8) cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<8>, p);
-    else if (lph == 16) cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<16>, p);
-    else cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<32>, p);
+    else if (lph == 1) go(std::integral_constant<int, 1>{});
+    else if (lph == 2) go(std::integral_constant<int, 2>{});
+    else if (lph == 4) go(std::integral_constant<int, 4>{});
+    else if (lph == 8) go(std::integral_constant<int, 8>{});
+    else if (lph == 16) go(std::integral_constant<int, 16>{});
+    else go(std::integral_constant<int, 32>{});
     return check_launch("qk_norm_rope_kernel");
 }
