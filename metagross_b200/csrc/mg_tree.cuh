@@ -105,7 +105,15 @@ __device__ __forceinline__ int scale_exponent(float s) {
 // The part of 2^e that the conversion's one fp16 FMA can hold: its offset of
 // 1152 * 2^e has to fit as well.  Scales of 64 and more need a second step.
 __device__ __forceinline__ int fma_exponent(int e) { return e > 5 ? 5 : e; }
+__device__ __forceinline__ float rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ float2 unpack_half2(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
 __device__ __forceinline__ uint32_t half_bits(float x) {
     return static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x)));
 }

@@ -151,9 +151,10 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
 
     // one group of 16 keys: kfrag(nt, s) and vfrag(j) give the fragments, ks
     // the score factor and vm the probability factor of this lane's keys
-    // (2c, 2c+1, 2c+8, 2c+9), seen(rt, u, i) whether row and key meet
-    // (uni: the four are the same, ks is positive and every key is seen)
-    auto attend = [&](auto&& kfrag, auto&& vfrag, const float (&ks)[4], const float (&vm)[4], auto&& seen, auto uni) {
+    // (2c, 2c+1, 2c+8, 2c+9), ivm its reciprocal, seen(rt, u, i) whether row and key
+    // meet (uni: the four are the same, ks is positive and every key is seen)
+    auto attend = [&](auto&& kfrag, auto&& vfrag, const float (&ks)[4], const float (&vm)[4], const float (&ivm)[4],
+                      auto&& seen, auto uni) {
         constexpr bool kUni = decltype(uni)::value;
         float s[RT][2][4];
 #pragma unroll
@@ -172,7 +173,8 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 for (int rt = 0; rt < RT; ++rt) mma_16816(s[rt][nt], qf[rt][st], b0, b1);
             }
         uint32_t pf[RT][4];
-        const float lvm = kUni ? __log2f(vm[0]) : 0.0f, ivm = kUni ? __frcp_rn(vm[0]) : 1.0f;
+        const float lvm = kUni ? __log2f(vm[0]) : 0.0f;
+        const float iuni = kUni ? ivm[0] : 1.0f;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float mx[2] = {-INFINITY, -INFINITY};
@@ -190,13 +192,14 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
                 mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
             }
-            // the reference maximum moves only when a score passes it by 2^8
-            // (probabilities up to 2^8 keep their precision in fp16): rescaling
-            // the output is rare, and skipped by the whole warp
-            if (__any_sync(0xffffffffu, mx[0] > m[rt][0] + 8.0f || mx[1] > m[rt][1] + 8.0f)) {
+            // The reference is set 2^6 below the largest score and moves only when
+            // a score passes it by 2^14: rescaling the output is rare, and skipped
+            // by the whole warp; a probability times the V scale's mantissa (below
+            // 2) stays inside fp16, and one of 2^-31 of the largest still counts.
+            if (__any_sync(0xffffffffu, mx[0] > m[rt][0] + 14.0f || mx[1] > m[rt][1] + 14.0f)) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const float mn = fmaxf(m[rt][u], mx[u]);
+                    const float mn = fmaxf(m[rt][u], mx[u] - 6.0f);
                     const float f = mn == -INFINITY ? 1.0f : ex2(m[rt][u] - mn);
                     m[rt][u] = mn;
                     l[rt][u] *= f;
@@ -210,26 +213,28 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const float ref = m[rt][u] == -INFINITY ? 0.0f : m[rt][u];
+                // Probabilities go to fp16 for the product with V, half a unit in
+                // 2^11 each.  The sum (fp32) takes them as rounded, so that the
+                // error of a row that one key dominates cancels.
                 if constexpr (kUni) {
                     // the V scale's mantissa goes into the exponent, and out of the sum again
                     const float off = lvm - ref;
                     float sum = 0.0f;
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt) {
-                        const float p0 = ex2(fmaf(s[rt][nt][2 * u], ks[0], off));
-                        const float p1 = ex2(fmaf(s[rt][nt][2 * u + 1], ks[0], off));
-                        sum += p0 + p1;
-                        pf[rt][nt * 2 + u] = pack_half2(p0, p1);
+                        pf[rt][nt * 2 + u] = pack_half2(ex2(fmaf(s[rt][nt][2 * u], ks[0], off)),
+                                                        ex2(fmaf(s[rt][nt][2 * u + 1], ks[0], off)));
+                        const float2 pr = unpack_half2(pf[rt][nt * 2 + u]);
+                        sum += pr.x + pr.y;
                     }
-                    l[rt][u] = fmaf(sum, ivm, l[rt][u]);
+                    l[rt][u] = fmaf(sum, iuni, l[rt][u]);
                 } else {
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt) {
                         const float p0 = ex2(s[rt][nt][2 * u] - ref), p1 = ex2(s[rt][nt][2 * u + 1] - ref);
-                        l[rt][u] += p0 + p1;
-                        // probabilities go to fp16 for the product with V (half a
-                        // unit in 2^11 each); their sum stays in fp32
                         pf[rt][nt * 2 + u] = pack_half2(p0 * vm[nt * 2], p1 * vm[nt * 2 + 1]);
+                        const float2 pr = unpack_half2(pf[rt][nt * 2 + u]);
+                        l[rt][u] = fmaf(pr.x, ivm[nt * 2], fmaf(pr.y, ivm[nt * 2 + 1], l[rt][u]));
                     }
                 }
             }
@@ -330,8 +335,8 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
     const int wt = 16 * warp;
     int jp = j0;           // first tile after the paged groups of this warp
     bool some_big = false;  // a group had a V scale of 64 or more and is left for later
-    // (or one below 2^-60, whose mantissa has no useful reciprocal)
-    auto big = [](float v) { return v >= 64.0f || v < 0x1p-60f; };
+    // (or one below 2^-20, whose exponent does not fit either)
+    auto big = [](float v) { return v >= 64.0f || v < 0x1p-20f; };
     {
         const int lim = whole - wt - 16;
         const int jend = lim < 0 ? j0 : min(j1, lim / kTreeTile + 1);
@@ -352,13 +357,14 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                     some_big = true;
                     continue;
                 }
-                float ks[4], vm[4];
+                float ks[4], vm[4], ivm[4];
                 VScale vsc[2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float v = cur.vs[UNI ? 0 : i];
                     ks[i] = cur.ks[UNI ? 0 : i] * p.scale_log2;
                     vm[i] = v * pow2f(-scale_exponent(v));
+                    ivm[i] = rcp(vm[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                            b0 = code_v(cur.v[0][w], cur.v[1][w], e, vsc[0]);
                            b1 = code_v(cur.v[2][w], cur.v[3][w], e, vsc[1]);
                        },
-                       ks, vm, [](int, int, int) { return true; }, std::integral_constant<bool, UNI>{});
+                       ks, vm, ivm, [](int, int, int) { return true; }, std::integral_constant<bool, UNI>{});
             }
             jp = jend;
         }
@@ -379,14 +385,14 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
     // ---- groups with staged rows, and the drafted tokens: fragments of halves
     bool bad = false;
     uint32_t kh[2][D / 8] = {}, vh[4][D / 16] = {};
-    auto half_groups = [&](const float (&ks)[4], const float (&vm)[4], auto&& seen) {
+    auto half_groups = [&](const float (&ks)[4], const float (&vm)[4], const float (&ivm)[4], auto&& seen) {
         attend([&](int nt, int s, uint32_t& b0, uint32_t& b1) { half_pair<KV4>(kh[nt], s, b0, b1); },
                [&](int jj, uint32_t& b0, uint32_t& b1) {
                    const uint32_t sel = (jj & 1) ? 0x7632 : 0x5410;
                    b0 = prmt(vh[0][jj >> 1], vh[1][jj >> 1], sel);
                    b1 = prmt(vh[2][jj >> 1], vh[3][jj >> 1], sel);
                },
-               ks, vm, seen, std::false_type{});
+               ks, vm, ivm, seen, std::false_type{});
     };
     auto clear_half = [&]() {
 #pragma unroll
@@ -410,7 +416,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
             if (!__any_sync(0xffffffffu, big(scale_at(p.v_scales, page_of(key), slot_of(key))))) continue;
         }
         clear_half();
-        float ks[4], vm[4];
+        float ks[4], vm[4], ivm[4];
         // a code as a half: its integer value; K's scale goes into the score,
         // V's exponent into the half and its mantissa into the probability
         auto half_code = [&](const uint32_t* w, int i) -> uint32_t {  // elements 2i, 2i + 1
@@ -443,14 +449,19 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
         for (int i = 0; i < 4; ++i) {
             const int tk = tok0 + 2 * c + (i & 1) + 8 * (i >> 1);
             ks[i] = p.scale_log2;
-            vm[i] = 1.0f;
+            vm[i] = ivm[i] = 1.0f;
             if (tk < whole) {
                 const int32_t pg = page_of(tk);
                 const float vs = scale_at(p.v_scales, pg, slot_of(tk));
                 ks[i] = scale_at(p.k_scales, pg, slot_of(tk)) * p.scale_log2;
                 const int e2 = scale_exponent(vs);
-                vm[i] = vs * pow2f(-e2);
-                const uint32_t f = half_bits(pow2f(e2)) * 0x10001u;
+                // scales down to 2^-27 go into the probability, smaller ones are zero
+                const bool none = fabsf(vs) < 0x1p-27f;
+                if (!none) {
+                    vm[i] = vs * pow2f(-e2);
+                    ivm[i] = rcp(vm[i]);
+                }
+                const uint32_t f = none ? 0u : half_bits(pow2f(e2)) * 0x10001u;
                 uint32_t w[F::VW];
                 ldg_words(w, row_at(p.v_pool, pg, slot_of(tk)) + g * (F::VW * 4));
 #pragma unroll
@@ -461,7 +472,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 keep_finite(vh[i]);
             }
         }
-        half_groups(ks, vm, [&](int, int, int key) { return tok0 + 2 * c + (key & 1) + 8 * (key >> 1) < n; });
+        half_groups(ks, vm, ivm, [&](int, int, int key) { return tok0 + 2 * c + (key & 1) + 8 * (key >> 1) < n; });
     }
     // drafted tokens; without a mask none past the row tile's last token is seen
     const int tmax = min(nd, p.mask ? nd : (min(row0 + BM, rows) - 1) / p.G + 1);
@@ -485,7 +496,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 keep_finite(vh[i]);
             }
         }
-        half_groups(ks1, ones, [&](int rt, int uu, int key) {
+        half_groups(ks1, ones, ones, [&](int rt, int uu, int key) {
             const int u = u0 + 2 * c + (key & 1) + 8 * (key >> 1);
             return tok[rt][uu] >= 0 && u < tmax && tree_sees(p, b, tok[rt][uu], u);
         });

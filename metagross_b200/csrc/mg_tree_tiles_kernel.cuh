@@ -40,12 +40,11 @@ namespace mg {
 constexpr uint32_t kTilesTries = 1u << 17;  // attempts of a bounded wait
 constexpr uint32_t kTilesNap = 100;         // ns between the attempts of a role with time to spare
 constexpr float kUnset = -1e30f;            // reference of a row that has seen no key
-// A row's reference is set 2^kRoom above its largest score so far and moves when a
-// score passes it by 2^kSlack: the probability times the V scale's mantissa
-// (below 2) stays inside fp16, and the room below, 2^10 of full precision under
-// the largest probability, keeps small ones exact enough (their sum is fp32 and
-// unrounded).  A large jump between tiles, 2^18 in all, is thus no event.
-constexpr float kSlack = 14.5f, kRoom = 4.0f;
+// A row's reference is its largest score so far (to the next whole number) and
+// moves when a score passes it by 2^kSlack: the probability times the V scale's
+// mantissa (below 2) stays inside fp16, and one of 2^-24 of the largest still
+// counts (the sum is fp32 and unrounded).
+constexpr float kSlack = 14.9f;
 
 template <bool KV4, int D>
 struct TilesCfg {
@@ -507,7 +506,7 @@ __global__ void __launch_bounds__(TilesCfg<KV4, D>::THREADS, 1) tree_tiles_kerne
                 }
                 float f = 1.0f;
                 if (mx > kSlack) {
-                    top += kRoom;
+                    top = ceilf(top);  // whole: the factor between two is exact in fp16
                     f = ex2(-nm - top);  // 0 from an unset reference
                     nm = -top;
                 }
