@@ -431,7 +431,8 @@ MG_API mg_status mg_tree_plan(const mg_cache_layout* layout, const int32_t* seq_
                               int32_t batch, int32_t max_draft, int32_t num_q_heads, void* plan, int64_t plan_bytes,
                               int32_t* dev_status, mg_stream_t stream);
 
-/* The attention of one layer.  fp16 staging; head_dim 64 or 128; out fp16
+/* The attention of one layer.  fp16 staging; head_dim 64 or 128; contexts
+ * below 2^26 tokens ((max_blocks + 1) * page_size); out fp16
  * [batch, max_draft, num_q_heads, D].  workspace: mg_tree_workspace_bytes()
  * bytes, 16-byte aligned, no initial contents; calls that share one must not
  * overlap on the device.  A plan made for other shapes sets

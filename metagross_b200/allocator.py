@@ -55,7 +55,8 @@ class BlockAllocator:
 
 
 class DeviceBlockAllocator:
-    """LIFO page stack in device memory (int32 free_stack [N], n_free [1], in_use [N])."""
+    """LIFO page stack in device memory (int32 free_stack [N], n_free [1], in_use [N]: the
+    sequences that hold each page, above 1 only after ``BatchedPagedKVCache.fork``)."""
 
     def __init__(self, num_pages: int, device="cuda"):
         if num_pages <= 0:

@@ -393,7 +393,7 @@ extern "C" mg_status mg_tree_attention(const mg_cache_layout* L, const mg_layer_
         else i4 ? launch_tree_tiles<true, 128>(p, g, s) : launch_tree_tiles<false, 128>(p, g, s);
     } else if (L->head_dim == 64) i4 ? launch_tree_rows<true, 64>(p, g, s) : launch_tree_rows<false, 64>(p, g, s);
     else i4 ? launch_tree_rows<true, 128>(p, g, s) : launch_tree_rows<false, 128>(p, g, s);
-    st = check_launch("tree_rows_kernel");
+    st = check_launch(g.tiles ? "tree_tiles_kernel" : "tree_rows_kernel");
     if (st != MG_OK) return st;
     const int64_t tasks = static_cast<int64_t>(p.T) * d->num_q_heads * batch;
     const int64_t blocks = (tasks + kJoinThreads / 32 - 1) / (kJoinThreads / 32);

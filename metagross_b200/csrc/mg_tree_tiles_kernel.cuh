@@ -40,11 +40,14 @@ namespace mg {
 constexpr uint32_t kTilesTries = 1u << 17;  // attempts of a bounded wait
 constexpr uint32_t kTilesNap = 100;         // ns between the attempts of a role with time to spare
 constexpr float kUnset = -1e30f;            // reference of a row that has seen no key
-// A row's reference is its largest score so far (to the next whole number) and
-// moves when a score passes it by 2^kSlack: the probability times the V scale's
-// mantissa (below 2) stays inside fp16, and one of 2^-24 of the largest still
-// counts (the sum is fp32 and unrounded).
-constexpr float kSlack = 14.9f;
+// A row's reference is set 2^kBelow (and up to twice that) below its largest score
+// so far and moves when a score passes it by 2^kSlack: the probability times the V
+// scale's mantissa (below 2) stays inside fp16, probabilities of 2^-18 of the largest
+// keep their 11 bits and those of 2^-28 still count (the sum is fp32 and unrounded).
+// Moving costs a warp about a tile's time: with the reference 2^4 above the maximum a
+// chunk of 512 tokens over 3841 takes 827 us for 841 at the maximum and 869 here, but
+// there rows that one key dominates lose their tail.
+constexpr float kSlack = 14.99f, kBelow = 4.0f;
 
 template <bool KV4, int D>
 struct TilesCfg {
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(TilesCfg<KV4, D>::THREADS, 1) tree_tiles_kerne
                 }
                 float f = 1.0f;
                 if (mx > kSlack) {
-                    top = ceilf(top);  // whole: the factor between two is exact in fp16
+                    top = floorf(top - kBelow);  // whole: the factor between two is exact in fp16
                     f = ex2(-nm - top);  // 0 from an unset reference
                     nm = -top;
                 }

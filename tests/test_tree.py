@@ -137,3 +137,11 @@ def test_qk_norm_refusals(lib):
         rc, err = call(**kw)
         assert rc == 1 and text in err, (kw, err)
     assert call(rows=0)[0] == 0
+
+
+@pytest.mark.parametrize("page,blocks,fits", [(16, (1 << 22) - 2, True), (16, (1 << 22) - 1, False), (64, 1 << 20, False)])
+def test_contexts_of_2_to_the_26_tokens_are_refused(lib, page, blocks, fits):
+    lay = Layout(0, 1, page, 4, 64, blocks, 1 << 23)
+    size = lib.mg_tree_plan_bytes(ctypes.byref(lay), 2, 4, 32)
+    assert (size > 0) == fits
+    assert fits or b"2^26" in lib.mg_last_error()
