@@ -44,10 +44,11 @@ constexpr float kUnset = -1e30f;            // reference of a row that has seen 
 // so far and moves when a score passes it by 2^kSlack: the probability times the V
 // scale's mantissa (below 2) stays inside fp16, probabilities of 2^-18 of the largest
 // keep their 11 bits and those of 2^-28 still count (the sum is fp32 and unrounded).
-// Moving costs a warp about a tile's time: with the reference 2^4 above the maximum a
-// chunk of 512 tokens over 3841 takes 827 us for 841 at the maximum and 869 here, but
-// there rows that one key dominates lose their tail.
-constexpr float kSlack = 14.99f, kBelow = 4.0f;
+// Moving is slow, so when a warp does it every row that rose by 2^kRefresh over its
+// reference takes part: eight chunks of 512 tokens over 3000 to 5000 tokens, two
+// layers, 857 us (871 when only those past 2^kSlack do).  With the reference at the
+// maximum it is 841, but then rows that one key dominates lose their tail.
+constexpr float kSlack = 14.99f, kBelow = 4.0f, kRefresh = 6.0f;
 
 template <bool KV4, int D>
 struct TilesCfg {
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(TilesCfg<KV4, D>::THREADS, 1) tree_tiles_kerne
                     top = fmaxf(top, front(k + 1, y, 0.0f));
                 }
                 float f = 1.0f;
-                if (mx > kSlack) {
+                if (mx > kRefresh) {
                     top = floorf(top - kBelow);  // whole: the factor between two is exact in fp16
                     f = ex2(-nm - top);  // 0 from an unset reference
                     nm = -top;
