@@ -13,7 +13,10 @@
 // targets held (their block-table rows are still needed for the order in
 // which pages go back, so nothing of them is overwritten yet);
 // fork_share_kernel shares the pages and copies the tails of every layer.
-// Bound: the tail bytes (read and write) at HBM rate, or the two launches.
+// Bound: the two launches (9 us for a few targets, 10 for 64 in 22 layers of 4
+// heads), then the latency of a CTA's one short copy (groups of four loads in
+// flight): 256 prefixes that cut a page, 12 layers of 12 heads of 64, 32 us with
+// 102 MB moved, 3.2 TB/s.
 #include "mg_alloc_step.cuh"
 #include "mg_common.cuh"
 
@@ -149,7 +152,9 @@ __global__ void __launch_bounds__(kForkThreads) fork_release_kernel(ForkParams p
                 atomicAdd(&p.in_use[page], 1);
                 flag(p.status, MG_DEV_DOUBLE_FREE);
             } else if (holders == 1) {
-                p.free_stack[top + atomicAdd(&p.ws[1], 1)] = page;
+                const int at = top + atomicAdd(&p.ws[1], 1);
+                if (at < p.num_pages) p.free_stack[at] = page;
+                else flag(p.status, MG_DEV_DOUBLE_FREE);  // more free pages than there are: the stack was not ours
             }
         }
     }
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(kForkThreads) fork_release_kernel(ForkParams p
     __syncthreads();
     if (!s_last) return;
     __threadfence();
-    const int released = *(volatile int32_t*)&p.ws[1];
+    const int released = static_cast<int>(min(static_cast<int64_t>(*(volatile int32_t*)&p.ws[1]), p.num_pages - *p.n_free));
     if (released > 0) push_released(p, released);
     __syncthreads();
     if (threadIdx.x == 0) p.ws[0] = p.ws[1] = 0;

@@ -12,9 +12,15 @@
 // way.  Codes become fp16 by exponent insertion and one fp16 FMA.
 //
 // Why: with R rows a (sequence, kv head) reads 2 D bits / 8 bytes and does
-// 4 R D products per key; up to R = 32 the loads are the bound on B200, and the
-// conversion of a key (paid once per 16 RT rows here) is the largest part of
-// the instructions.
+// 4 R D products per key; for so few rows the conversion of a key (paid once per
+// 16 RT rows here) is the largest part of the work, and a trip of the codes
+// through shared memory would add to it.
+// Measured (one B200, a layer): 32 INT8 contexts of ~1012 tokens, 12 heads of 64, 8
+// drafted tokens: 25.6 us with its join, 2.0 TB/s; 200 log-normal INT4 contexts up to
+// 32768, 5 drafted tokens for 8 heads each: 194 us.  Bound: ~330 dependent
+// instructions per warp and 16 keys at 2.6 warps per scheduler (issue slots 37 %
+// used, DRAM 28 %, tensor pipe 13 %).  More CTAs per SM spill; loads further ahead
+// and L2 prefetch were slower.
 #pragma once
 
 #include <type_traits>

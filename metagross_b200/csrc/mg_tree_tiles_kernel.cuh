@@ -30,6 +30,11 @@
 //
 // Bound: the exponentials (16 per clock and SM): 128 x 128 scores take 1024
 // clocks, the products 512 (D = 64) or 1024; for few rows the conversion and loads.
+// Measured (one B200): about 2800 clocks a tile, from the latency of a softmax warp's
+// chain (issue slots 50 % used, exponentials at 35 % of their rate, tensor pipe 16 %);
+// 8 chunks of 512 tokens over 3000 to 5000, 32 q / 4 kv heads of 64, INT8: 428 us a
+// layer, 334 TFLOP/s; 64 contexts U[128, 2048] with trees of 16, INT4: 80 us a layer,
+// of which some 15 are the prologue, first tile, drafted tile and join.
 #pragma once
 
 #include "mg_tcgen05.cuh"
