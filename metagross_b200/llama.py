@@ -231,6 +231,15 @@ class LlamaDecoder:
         mask = tree_mask(parents).to(dev).expand(B, T, T)
         parents = torch.as_tensor(parents).long().to(dev).expand(B, T)
         depth = tree_depths(mask)
+        # one wait for the three: nothing below may index past its table
+        above = (parents - torch.arange(T, device=dev)).max()
+        end, above, low, high = torch.stack([(self.pos[:, None] + depth).max(), above, drafts.min(), drafts.max()]).tolist()
+        if above >= 0:
+            raise ValueError("a token's parent must have a smaller index than the token")
+        if end >= self.max_len:
+            raise ValueError(f"drafts reach position {end}, past max_len={self.max_len}")
+        if low < 0 or high >= s.vocab:
+            raise ValueError(f"drafts must be token ids in [0, {s.vocab})")
         hq, hkv, D, L = s.heads, s.kv_heads, s.head_dim, s.layers
         pos = (self.pos[:, None] + depth).reshape(-1)
         x = self.w["embed"][drafts].reshape(B * T, s.hidden)

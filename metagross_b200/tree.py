@@ -13,12 +13,14 @@ import torch
 
 def tree_mask(parents) -> torch.Tensor:
     """Bool mask [..., T, T] of a parent list or tensor [..., T]: True where
-    token t sees token u, that is u is t or one of its ancestors."""
+    token t sees token u, that is u is t or one of its ancestors.  A parent that is not
+    below its token is refused (on the device, where looking would wait: counts as none)."""
     p = torch.as_tensor(parents).long()
     T = p.shape[-1]
     i = torch.arange(T, device=p.device)
     if p.device.type == "cpu" and bool((p >= i).any()):
         raise ValueError("a token's parent must have a smaller index than the token")
+    p = torch.where(p < i, p, -1)
     # seen: ancestors at distances below reach; up: the ancestor at distance reach
     seen = (i[:, None] == i).expand(*p.shape, T)
     up, reach = p, 1

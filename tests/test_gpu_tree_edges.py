@@ -128,3 +128,22 @@ def test_a_plan_of_other_shapes_is_flagged(T):
     torch.cuda.synchronize()
     assert int(c.status.item()) == 0x80
     assert (out == 7.0).all()
+
+
+def test_verify_refuses_what_would_leave_its_tables():
+    from test_gpu_verify import B, decoder, prompt
+
+    d = decoder()  # up to 96 tokens
+    d.prefill(prompt(n=90))  # positions 90 .. 95 are left
+    ids = torch.zeros(B, 7, dtype=torch.long, device="cuda")
+    chain = list(range(-1, 6))
+    with pytest.raises(ValueError, match="max_len"):
+        d.verify(ids, chain)
+    with pytest.raises(ValueError, match="parent"):
+        d.verify(ids, torch.tensor([-1, 0, 9, 0, 0, 0, 0], device="cuda"))
+    for bad in (-1, 64):
+        with pytest.raises(ValueError, match="token ids"):
+            d.verify(torch.full_like(ids, bad), [-1, 0, 0, 0, 0, 0, 0])
+    tokens, n = d.verify(ids, [-1, 0, 0, 0, 0, 0, 0])  # wide, but short
+    d.cache.check()
+    assert (n >= 1).all()
