@@ -243,11 +243,12 @@ TreeGeom tree_geometry(const mg_cache_layout& L, int64_t batch, int64_t T, int64
     const int64_t rows = T * (Hq / L.num_kv_heads);
     int occ;
     // Above 48 rows the tensor-core tile kernel, whose time hardly depends on the
-    // rows (one B200, us per call): head_dim 64, 64 sequences of 1000 tokens, 4 kv
-    // heads, INT8: 32 rows 34 (row kernel) / 61 (tile kernel), 64 rows 65 / 67, 128
-    // rows 93 / 85; 200 sequences of 3000, INT4: 32 rows 178 / 221, 40 rows 267 /
-    // 226, 128 rows 548 / 254; head_dim 128, 12 sequences of 3000, INT8: 48 rows 65 /
-    // 76, 64 rows 113 / 77, 128 rows 190 / 86.
+    // rows (one B200, us per call, row kernel / tile kernel): head_dim 64, 64 sequences
+    // of 1000 tokens, 4 kv heads, INT8: 32 rows 31 / 62, 40 rows 56 / 63, 64 rows 61 /
+    // 68, 128 rows 85 / 86, 256 rows 162 / 93; 200 sequences of 3000, INT4: 32 rows 158 /
+    // 215, 40 rows 234 / 218, 64 rows 246 / 221, 128 rows 477 / 239; head_dim 128, 12
+    // sequences of 3000, 8 kv heads, INT8: 40 rows 60 / 72, 64 rows 107 / 74, 128 rows
+    // 177 / 80.
     g.tiles = rows > 48;
     if (g.tiles) {
         g.tile = kTilesKeys;
