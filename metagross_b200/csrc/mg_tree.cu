@@ -191,14 +191,16 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(TreeParams p, i
 #pragma unroll 4
             for (int k = 0; k < s.y; ++k) {
                 const float2 w = ml[k * step];
-                // a piece without a finite score weighs nothing, but its NaN sum goes through
+                // a piece without a finite score weighs nothing, but its NaN sum goes through;
+                // so does an infinity or NaN that a row saw in V, which a weight of 0 would turn
+                // into NaN (as in the unsplit kernels, where it is added after the weighting)
                 const float f = mx == -INFINITY ? 0.0f : ex2(w.x - mx);
                 ls += f * w.y;
                 float x[V];
                 if constexpr (V == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(po + k * step * D);
                 else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(po + k * step * D);
 #pragma unroll
-                for (int e = 0; e < V; ++e) a[e] += f * x[e];
+                for (int e = 0; e < V; ++e) a[e] += isfinite(x[e]) ? f * x[e] : x[e];
             }
             const float inv = ls > 0.0f || isnan(ls) ? 1.0f / ls : 0.0f;
 #pragma unroll

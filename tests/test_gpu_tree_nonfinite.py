@@ -41,3 +41,49 @@ def test_a_query_that_is_not_finite(kv, d, T, value):
     other = torch.ones(out.shape[:3], dtype=torch.bool, device="cuda")
     other[:, 1, 5] = False
     assert ((out.double() - ref).abs() <= bar)[other].all()
+
+
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("lens,cut", [([3000], True), ([20] * 700, False), ([0] * 700, False)])
+def test_an_infinity_in_a_value_of_vanishing_weight(T, lens, cut):
+    """The drafted keys score e^-300 of the cached ones, less than fp32 can hold: the row that sees an infinity
+    gets it all the same, whether the drafted tokens are a piece of their own or not."""
+    c = make_cache(lens, 2, 64)
+    c.k_pool.zero_()  # every cached score is 0
+    c.staging_k.zero_()
+    q, k, v = drafts(c, T, 8)
+    q.zero_()
+    k.zero_()
+    q[..., 0], k[..., 0] = 1.0, -300.0
+    assert is_cut(c.plan_tree(T, 8)) == cut
+    clean = c.attend_tree(0, q, k, v, scale=1.0)
+    v[:, 1, :, 5], v[:, 1, :, 6], v[:, 1, :, 7] = math.inf, -math.inf, math.nan
+    out = c.attend_tree(0, q, k, v, scale=1.0)
+    torch.cuda.synchronize()
+    c.check()
+    assert torch.equal(out[:, :1], clean[:, :1])
+    assert (out[:, 1:, :, 5] == math.inf).all() and (out[:, 1:, :, 6] == -math.inf).all()
+    assert out[:, 1:, :, 7].isnan().all()
+    keep = [i for i in range(64) if i not in (5, 6, 7)]
+    assert torch.equal(out[..., keep], clean[..., keep])
+
+
+@pytest.mark.parametrize("T", [3, 40])
+def test_an_infinity_in_a_staged_value_of_vanishing_weight(T):
+    """The same where the staged rows fill the last piece of the context."""
+    c = make_cache([47 * 64 - 1], 2, 64, page=64)
+    c.k_pool.zero_()
+    c.staging_k.zero_()
+    c.staging_k[..., 0] = -300.0
+    q, k, v = drafts(c, T, 8)
+    q.zero_()
+    k.zero_()
+    q[..., 0] = 1.0
+    clean = c.attend_tree(0, q, k, v, scale=1.0)
+    c.staging_v[:, :, 9, :, 5], c.staging_v[:, :, 9, :, 6] = math.inf, -math.inf
+    out = c.attend_tree(0, q, k, v, scale=1.0)
+    torch.cuda.synchronize()
+    c.check()
+    assert (out[..., 5] == math.inf).all() and (out[..., 6] == -math.inf).all()
+    keep = [i for i in range(64) if i not in (5, 6)]
+    assert torch.equal(out[..., keep], clean[..., keep])
