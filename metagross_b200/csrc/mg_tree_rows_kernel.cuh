@@ -31,6 +31,8 @@ namespace mg {
 
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
+// what a group of 16 keys is to the attention step
+enum { kPagedGroup, kUniGroup, kTinyGroup };
 
 template <bool KV4, int D>
 struct RowsFmt {
@@ -158,10 +160,11 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
     // one group of 16 keys: kfrag(nt, s) and vfrag(j) give the fragments, ks
     // the score factor and vm the probability factor of this lane's keys
     // (2c, 2c+1, 2c+8, 2c+9), ivm its reciprocal, seen(rt, u, i) whether row and key
-    // meet (uni: the four are the same, ks is positive and every key is seen)
+    // meet (kUniGroup: the four are the same, ks is positive and every key is seen;
+    // kTinyGroup: ivm may be 0, for a key whose factor is too small to divide out)
     auto attend = [&](auto&& kfrag, auto&& vfrag, const float (&ks)[4], const float (&vm)[4], const float (&ivm)[4],
-                      auto&& seen, auto uni) {
-        constexpr bool kUni = decltype(uni)::value;
+                      auto&& seen, auto kind) {
+        constexpr bool kUni = decltype(kind)::value == kUniGroup, kTiny = decltype(kind)::value == kTinyGroup;
         float s[RT][2][4];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -240,7 +243,13 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                         const float p0 = ex2(s[rt][nt][2 * u] - ref), p1 = ex2(s[rt][nt][2 * u + 1] - ref);
                         pf[rt][nt * 2 + u] = pack_half2(p0 * vm[nt * 2], p1 * vm[nt * 2 + 1]);
                         const float2 pr = unpack_half2(pf[rt][nt * 2 + u]);
-                        l[rt][u] = fmaf(pr.x, ivm[nt * 2], fmaf(pr.y, ivm[nt * 2 + 1], l[rt][u]));
+                        if constexpr (kTiny) {
+                            const float i0 = ivm[nt * 2], i1 = ivm[nt * 2 + 1];
+                            l[rt][u] = fmaf(i0 == 0.0f ? p0 : pr.x, i0 == 0.0f ? 1.0f : i0,
+                                            fmaf(i1 == 0.0f ? p1 : pr.y, i1 == 0.0f ? 1.0f : i1, l[rt][u]));
+                        } else {
+                            l[rt][u] = fmaf(pr.x, ivm[nt * 2], fmaf(pr.y, ivm[nt * 2 + 1], l[rt][u]));
+                        }
                     }
                 }
             }
@@ -382,7 +391,8 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                            b0 = code_v(cur.v[0][w], cur.v[1][w], e, vsc[0]);
                            b1 = code_v(cur.v[2][w], cur.v[3][w], e, vsc[1]);
                        },
-                       ks, vm, ivm, [](int, int, int) { return true; }, std::integral_constant<bool, UNI>{});
+                       ks, vm, ivm, [](int, int, int) { return true; },
+                       std::integral_constant<int, UNI ? kUniGroup : kPagedGroup>{});
             }
             jp = jend;
         }
@@ -398,7 +408,7 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                    b0 = prmt(vh[0][jj >> 1], vh[1][jj >> 1], sel);
                    b1 = prmt(vh[2][jj >> 1], vh[3][jj >> 1], sel);
                },
-               ks, vm, ivm, seen, std::false_type{});
+               ks, vm, ivm, seen, std::integral_constant<int, kTinyGroup>{});
     };
     auto clear_half = [&]() {
 #pragma unroll
@@ -461,13 +471,12 @@ __global__ void __launch_bounds__(kRowsThreads, rows_ctas_per_sm<D, RT>()) tree_
                 const float vs = scale_at(p.v_scales, pg, slot_of(tk));
                 ks[i] = scale_at(p.k_scales, pg, slot_of(tk)) * p.scale_log2;
                 const int e2 = scale_exponent(vs);
-                // scales down to 2^-27 go into the probability, smaller ones are zero
-                const bool none = fabsf(vs) < 0x1p-27f;
-                if (!none) {
-                    vm[i] = vs * pow2f(-e2);
-                    ivm[i] = rcp(vm[i]);
-                }
-                const uint32_t f = none ? 0u : half_bits(pow2f(e2)) * 0x10001u;
+                // a scale below 2^-27 leaves too few bits of the rounded probability for
+                // the sum, which takes the unrounded one; the key's part of the output is
+                // below 127 x 2^-27, where that error is far below the smallest half
+                vm[i] = vs * pow2f(-e2);
+                ivm[i] = fabsf(vs) < 0x1p-27f ? 0.0f : rcp(vm[i]);
+                const uint32_t f = half_bits(pow2f(e2)) * 0x10001u;
                 uint32_t w[F::VW];
                 ldg_words(w, row_at(p.v_pool, pg, slot_of(tk)) + g * (F::VW * 4));
 #pragma unroll

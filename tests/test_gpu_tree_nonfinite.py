@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_tree import context, drafts, make_cache, reference
+from test_gpu_tree import compare, context, drafts, make_cache, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,29 @@ def test_an_infinity_in_a_staged_value_of_vanishing_weight(T):
     assert (out[..., 5] == math.inf).all() and (out[..., 6] == -math.inf).all()
     keep = [i for i in range(64) if i not in (5, 6)]
     assert torch.equal(out[..., keep], clean[..., keep])
+
+
+@pytest.mark.parametrize("T", [1, 3, 6, 30])
+@pytest.mark.parametrize("scales,page", [("page", 16), ("token_head", 16), ("page", 24)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_values_of_a_few_of_the_smallest_halves(T, scales, page, mixed):
+    """V rows of 0 to 15 times 2^-24, whose scales lie below 2^-27: such keys count like any other, alone and
+    beside pages of ordinary values."""
+    from metagross_b200.batched import BatchedPagedKVCache
+
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n = [200, 31, 70]
+    c = BatchedPagedKVCache(1, 3, 2, 64, page_size=page, num_pages=40, max_blocks=16, kv_dtype="int8",
+                            scale_granularity=scales)
+    c.begin_step(torch.tensor(n, dtype=torch.int32))
+    k = torch.randn(3, 200, 2, 64, generator=g, device="cuda")
+    v = torch.randint(0, 16, (3, 200, 2, 64), generator=g, device="cuda") * 2.0 ** -24
+    if mixed:
+        v[:, page:2 * page] = torch.randn(3, page, 2, 64, generator=g, device="cuda")
+    c.append(0, k.half(), v.half())
+    c.check()
+    assert 0 < c.v_scales[0, c.block_tables[0, 0].long()].min() < 2.0 ** -27
+    q, kd, _ = drafts(c, T, 8)
+    vd = (torch.randint(0, 16, kd.shape, generator=g, device="cuda") * 2.0 ** -24).half()
+    out = compare(c, q, kd, vd)
+    assert mixed or (out.amax((2, 3)) >= 4 * 2.0 ** -24).all()  # the mean of the values is 7.5 units
