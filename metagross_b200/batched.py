@@ -128,7 +128,8 @@ class BatchedPagedKVCache:
         self._plan_ok = False
         self._plan_last = False  # the plan kernel is the cache's latest launch (nothing after it yet)
         self._lens_version = 0  # changes with the lengths or tables; a TreePlan of another version is stale
-        self._fork_ws = torch.zeros(2, dtype=torch.int32, device=self.device)
+        # as many pairs as there are targets; never replaced, since a captured fork keeps its address
+        self._fork_ws = torch.zeros(_get_C().fork_workspace_bytes(batch) // 4, dtype=torch.int32, device=self.device)
 
     # ------------------------------------------------------------------ steps
     def begin_step(self, n_new, plan: bool = False) -> None:
@@ -318,7 +319,10 @@ class BatchedPagedKVCache:
         Committed pages are shared and go back to the pool with their last holder; the exact
         rows after them are copied, or dequantized where lens cuts a committed page.  What dst
         held is released first.  src, dst, lens: lists or int32 tensors; a target may not be a
-        source or appear twice (device tensors: such pairs are skipped and ``check`` raises)."""
+        source or appear twice (device tensors: such pairs are skipped and ``check`` raises).
+        Like every call that changes the cache, forks of one cache run one after the other:
+        on one stream, or with streams that wait for each other.  It can be captured in a graph
+        (device ids); ``invalidate_plan`` after a replay, which moves the lengths on the device."""
         on_device = isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and src.is_cuda and dst.is_cuda
         if not on_device:
             s, d = (torch.as_tensor(x).flatten().tolist() for x in (src, dst))
@@ -328,19 +332,27 @@ class BatchedPagedKVCache:
                 raise ValueError(f"sequence ids must be in [0, {self.batch})")
             if len(set(d)) != len(d) or set(d) & set(s):
                 raise ValueError("a target may not be a source or appear twice")
+        self._fork(src, dst, lens)
+
+    def _fork(self, src, dst, lens) -> torch.Tensor:
+        """``fork`` without its checks of lists; returns the workspace, which holds a word per pair from
+        its third on until the next fork: nonzero where the pair was done."""
         ids = [torch.as_tensor(x, dtype=torch.int32, device=self.device).contiguous() for x in (src, dst)]
         if lens is not None:
             lens = torch.as_tensor(lens, dtype=torch.int32, device=self.device).contiguous()
         C = _get_C()
         need = C.fork_workspace_bytes(ids[0].numel()) // 4
-        if need > self._fork_ws.numel():
-            self._fork_ws = torch.zeros(need, dtype=torch.int32, device=self.device)
+        # more pairs than sequences (some of them are skipped) take a workspace of their own
+        ws = self._fork_ws
+        if need > ws.numel():
+            ws = torch.zeros(need, dtype=torch.int32, device=self.device)
         self._plan_ok = False
         self._lens_version += 1
         C.fork_sequences(self.allocator.free_stack, self.allocator.n_free, self.allocator.in_use, self.k_pool,
                          self.v_pool, self.k_scales, self.v_scales, self.staging_k, self.staging_v, self.block_tables,
-                         self.seq_lens, ids[0], ids[1], lens, self._fork_ws, self.status)
+                         self.seq_lens, ids[0], ids[1], lens, ws, self.status)
         self._plan_last = False
+        return ws
 
     def gather(self, layer: int, dtype=torch.float32, include_staging: bool = True):
         """Dequantized K, V of every sequence, packed: ([total, Hkv, D], [total, Hkv, D], cu_seqlens [B+1])."""
