@@ -217,9 +217,9 @@ class LlamaDecoder:
     def verify(self, drafts: torch.Tensor, parents) -> tuple[torch.Tensor, torch.Tensor]:
         """One step that checks a tree of drafted tokens per sequence.
 
-        drafts [B, T]: column 0 is the pending token (``ids``), the others are guesses of what
-        follows; parents [T] or [B, T]: each token's parent, below its own index (-1 for column
-        0).  Every token runs through the model at its depth's position.  A guess is accepted
+        drafts [B, T]: column 0 is the pending token (``ids``, or the caller's own choice in its
+        place: it is appended unchecked), the others are guesses of what follows; parents [T] or
+        [B, T]: each token's parent, below its own index (-1 for column 0 alone).  Every token runs through the model at its depth's position.  A guess is accepted
         if its parent is and the model's greedy token after the parent is the guess; the
         longest accepted path is appended to the cache and ``ids`` becomes the model's token
         after it.  Returns (tokens [B, T] of the path, in order, and their counts [B], >= 1)."""
@@ -231,11 +231,15 @@ class LlamaDecoder:
         mask = tree_mask(parents).to(dev).expand(B, T, T)
         parents = torch.as_tensor(parents).long().to(dev).expand(B, T)
         depth = tree_depths(mask)
-        # one wait for the three: nothing below may index past its table
-        above = (parents - torch.arange(T, device=dev)).max()
-        end, above, low, high = torch.stack([(self.pos[:, None] + depth).max(), above, drafts.min(), drafts.max()]).tolist()
+        # one wait for the five: nothing below may index past its table, nor accept a token without a check
+        col = torch.arange(T, device=dev)
+        above, least = (parents - col).max(), torch.where(col > 0, parents, 0).min()
+        end, above, least, low, high = torch.stack([(self.pos[:, None] + depth).max(), above, least, drafts.min(),
+                                                    drafts.max()]).tolist()
         if above >= 0:
             raise ValueError("a token's parent must have a smaller index than the token")
+        if least < 0:
+            raise ValueError("only column 0, the pending token, has no parent")
         if end >= self.max_len:
             raise ValueError(f"drafts reach position {end}, past max_len={self.max_len}")
         if low < 0 or high >= s.vocab:
