@@ -228,8 +228,11 @@ class LlamaDecoder:
         if B != self.batch or T < 1:
             raise ValueError(f"drafts must be [{self.batch}, at least 1]")
         drafts = drafts.to(dev)
+        parents = torch.as_tensor(parents).long()
+        if parents.shape not in ((T,), (1, T), (B, T)):
+            raise ValueError(f"parents must be [{T}] or [{B}, {T}], got {list(parents.shape)}")
         mask = tree_mask(parents).to(dev).expand(B, T, T)
-        parents = torch.as_tensor(parents).long().to(dev).expand(B, T)
+        parents = parents.to(dev).expand(B, T)
         depth = tree_depths(mask)
         # one wait for the five: nothing below may index past its table, nor accept a token without a check
         col = torch.arange(T, device=dev)

@@ -20,3 +20,16 @@ def test_a_second_root_is_refused():
             with pytest.raises(ValueError, match="column 0"):
                 d.verify(tree, p)
     assert torch.equal(d.ids, ids) and torch.equal(d.cache.seq_lens, lens)
+
+
+def test_parents_of_another_shape_are_refused():
+    d = decoder()
+    d.prefill(prompt())
+    tree = torch.zeros(B, 3, dtype=torch.long, device="cuda")
+    for parents in ([-1], [-1, 0], [-1, 0, 1, 2], [[-1, 0, 1]] * (B + 1), [[-1]] * B, [[[-1, 0, 1]] * B]):
+        with pytest.raises(ValueError, match="parents must be"):
+            d.verify(tree, parents)
+    assert d.cache.seq_lens.tolist() == [21] * B
+    for parents in ([-1, 0, 1], [[-1, 0, 1]], [[-1, 0, 1]] * B):
+        d.verify(tree, parents)
+    d.cache.check()
