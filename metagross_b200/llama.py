@@ -152,7 +152,8 @@ class LlamaDecoder:
         """q | k | v of the projection's rows, q and k (normalised and) rotated at positions pos."""
         C, w = _get_C(), self.w
         if self.s.qk_norm:
-            C.qk_norm_rope(qkv, w[f"{i}.qn"], w[f"{i}.kn"], pos, self.cos, self.sin, self.s.rms_eps, q, k, v)
+            C.qk_norm_rope(qkv, w[f"{i}.qn"], w[f"{i}.kn"], pos, self.cos, self.sin, self.s.rms_eps, q, k, v,
+                           self.cache.status)  # a position past the tables is reported by cache.check()
         else:
             C.rope_qkv(qkv, pos, self.cos, self.sin, q, k, v)
 

@@ -33,3 +33,16 @@ def test_parents_of_another_shape_are_refused():
     for parents in ([-1, 0, 1], [[-1, 0, 1]], [[-1, 0, 1]] * B):
         d.verify(tree, parents)
     d.cache.check()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_normed_decoder_past_its_tables_is_reported(captured):
+    d = decoder(qk_norm=True)  # up to 96 tokens
+    d.prefill(prompt(n=90))
+    if captured:
+        d.capture()
+    d.decode(7)  # six steps: positions 90 .. 95
+    d.cache.check()
+    d.decode(2)
+    with pytest.raises(RuntimeError, match="argument"):
+        d.cache.check()
