@@ -323,19 +323,24 @@ class BatchedPagedKVCache:
         Like every call that changes the cache, forks of one cache run one after the other:
         on one stream, or with streams that wait for each other.  It can be captured in a graph
         (device ids); ``invalidate_plan`` after a replay, which moves the lengths on the device."""
-        on_device = isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and src.is_cuda and dst.is_cuda
-        if not on_device:
-            s, d = (torch.as_tensor(x).flatten().tolist() for x in (src, dst))
-            if len(s) != len(d):
-                raise ValueError("src and dst must have the same length")
-            if any(not 0 <= x < self.batch for x in s + d):
-                raise ValueError(f"sequence ids must be in [0, {self.batch})")
-            if len(set(d)) != len(d) or set(d) & set(s):
-                raise ValueError("a target may not be a source or appear twice")
+        self._check_pairs(src, dst)
         self._fork(src, dst, lens)
 
+    def _check_pairs(self, src, dst) -> None:
+        """Refuse what ``fork`` cannot do, of pairs that the host can see."""
+        on_device = isinstance(src, torch.Tensor) and isinstance(dst, torch.Tensor) and src.is_cuda and dst.is_cuda
+        if on_device:
+            return
+        s, d = (torch.as_tensor(x).flatten().tolist() for x in (src, dst))
+        if len(s) != len(d):
+            raise ValueError("src and dst must have the same length")
+        if any(not 0 <= x < self.batch for x in s + d):
+            raise ValueError(f"sequence ids must be in [0, {self.batch})")
+        if len(set(d)) != len(d) or set(d) & set(s):
+            raise ValueError("a target may not be a source or appear twice")
+
     def _fork(self, src, dst, lens) -> torch.Tensor:
-        """``fork`` without its checks of lists; returns the workspace, which holds a word per pair from
+        """``fork`` without that check; returns the workspace, which holds a word per pair from
         its third on until the next fork: nonzero where the pair was done."""
         ids = [torch.as_tensor(x, dtype=torch.int32, device=self.device).contiguous() for x in (src, dst)]
         if lens is not None:

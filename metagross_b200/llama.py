@@ -284,11 +284,17 @@ class LlamaDecoder:
 
     def fork(self, src, dst) -> None:
         """Sequences dst become copies of sequences src: the cache (shared pages, copied exact
-        rows), the position and the pending token."""
-        self.cache.fork(src, dst)
-        src, dst = (torch.as_tensor(x).long().to(self.device) for x in (src, dst))
-        self.ids[dst] = self.ids[src]
-        self.pos[dst] = self.pos[src]
+        rows), the position and the pending token.  A pair that the cache skips (device ids)
+        changes none of them."""
+        self.cache._check_pairs(src, dst)
+        ws = self.cache._fork(src, dst, None)
+        src, dst = (torch.as_tensor(x, dtype=torch.int32, device=self.device).flatten().long() for x in (src, dst))
+        done = ws[2:2 + src.numel()] != 0
+        # pairs that the cache skipped write to a row past the last
+        dst = torch.where(done, dst, self.batch)
+        src = torch.where(done, src, 0)
+        for x in (self.ids, self.pos):
+            x.copy_(torch.cat([x, x[:1]]).index_copy(0, dst, x[src])[:-1])
 
     def capture(self) -> None:
         """Capture the decode step in a CUDA graph (after prefill)."""

@@ -46,3 +46,41 @@ def test_a_normed_decoder_past_its_tables_is_reported(captured):
     d.decode(2)
     with pytest.raises(RuntimeError, match="argument"):
         d.cache.check()
+
+
+def four():
+    """Four sequences of different lengths and pending tokens."""
+    d = decoder(batch=4)
+    d.prefill(prompt(4, n=40))
+    d.cache.truncate([32, 16], [1, 2])
+    d.pos.copy_(d.cache.seq_lens)
+    d.ids.copy_(torch.tensor([11, 12, 13, 14], device="cuda"))
+    return d
+
+
+def same(d, ids, lens):
+    assert d.ids.tolist() == ids and d.pos.tolist() == lens and d.cache.seq_lens.tolist() == lens
+
+
+def test_fork_copies_what_the_cache_copies():
+    """Device ids: a pair that the cache skips moves neither the position nor the pending token."""
+    dev = lambda *x: torch.tensor(x, device="cuda")  # noqa: E731
+    d = four()
+    d.fork(dev(0, 2), dev(2, 3))  # 2 is a source: only the second pair
+    same(d, [11, 12, 13, 13], [40, 32, 16, 16])
+    d = four()
+    d.fork(dev(0, 1), dev(3, 3))  # 3 twice: the first pair
+    same(d, [11, 12, 13, 11], [40, 32, 16, 40])
+    d = four()
+    d.cache.status.fill_(0x1)  # a refused step: nothing is done
+    d.fork(dev(0), dev(1))
+    same(d, [11, 12, 13, 14], [40, 32, 16, 40])
+
+
+def test_fork_skips_ids_out_of_range():
+    dev = lambda *x: torch.tensor(x, device="cuda")  # noqa: E731
+    d = four()
+    d.fork(dev(9, 0, -1, 1, 0), dev(2, 3, 3, 70000, -2))
+    same(d, [11, 12, 13, 11], [40, 32, 16, 40])
+    with pytest.raises(RuntimeError, match="argument"):
+        d.cache.check()
