@@ -278,9 +278,10 @@ class LlamaDecoder:
         c.begin_step(n)
         for i in range(L):
             c.append(i, k[i], v[i])
+        tokens = drafts.gather(1, path)  # before ids, which drafts may be a view of, changes
         self.ids.copy_(nxt.gather(1, best)[:, 0])
         self.pos += n
-        return drafts.gather(1, path), n
+        return tokens, n
 
     def fork(self, src, dst) -> None:
         """Sequences dst become copies of sequences src: the cache (shared pages, copied exact

@@ -84,3 +84,13 @@ def test_fork_skips_ids_out_of_range():
     same(d, [11, 12, 13, 11], [40, 32, 16, 40])
     with pytest.raises(RuntimeError, match="argument"):
         d.cache.check()
+
+
+def test_drafts_may_be_a_view_of_the_pending_tokens():
+    d = decoder()
+    d.prefill(prompt())
+    for _ in range(4):
+        pending = d.ids.clone()
+        tokens, n = d.verify(d.ids[:, None], [-1])
+        assert torch.equal(tokens[:, 0], pending) and (n == 1).all()
+        assert not torch.equal(d.ids, pending)
