@@ -287,7 +287,8 @@ class BatchedPagedKVCache:
         chunk of a prompt.  n_draft int32 [B]: drafted tokens of each sequence; later rows come
         out as zeros, as does a row that sees nothing.  The cache is not changed: append the
         accepted tokens afterwards.  plan: ``plan_tree``'s, shared by the layers of a step
-        (which then carries n_draft); without it the call makes its own."""
+        (which then carries n_draft); without it the call makes its own.  Scores, sums and
+        outputs are fp32; probabilities are rounded to fp16 for their product with V."""
         if q.dim() != 4 or q.shape[0] != self.batch or q.shape[3] != self.head_dim:
             raise ValueError(f"q must be [{self.batch}, drafted tokens, num_q_heads, {self.head_dim}], "
                              f"got {tuple(q.shape)}")

@@ -17,7 +17,7 @@
 // through shared memory would add to it.
 // Measured (one B200, a layer): 32 INT8 contexts of ~1012 tokens, 12 heads of 64, 8
 // drafted tokens: 25.6 us with its join, 2.0 TB/s; 200 log-normal INT4 contexts up to
-// 32768, 5 drafted tokens for 8 heads each: 194 us.  Bound: ~330 dependent
+// 32768, 5 drafted tokens for 8 heads each: 196 us.  Bound: ~330 dependent
 // instructions per warp and 16 keys at 2.6 warps per scheduler (issue slots 37 %
 // used, DRAM 28 %, tensor pipe 13 %).  More CTAs per SM spill; loads further ahead
 // and L2 prefetch were slower.

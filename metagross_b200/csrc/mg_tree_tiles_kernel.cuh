@@ -17,7 +17,9 @@
 //   maximum  a reference; 32 scores at a time are compared with it, and only when
 //            one passes it by a wide margin does the warp move it: sum, output and
 //            the tile's probabilities so far are rescaled in place.
-//   sum      fp32, of the unrounded probabilities.
+//   sum      fp32, of the unrounded probabilities.  The products take them rounded to
+//            fp16: relative error 2.9e-4 of the output, where the row kernel, which sums
+//            them as rounded at the price of unpacking every pair, has 2.2e-4.
 //
 // Roles (warpgroups; registers are moved to the softmax):
 //   0, 1     softmax of the even / odd tiles: S from tensor memory, P over it
@@ -32,9 +34,11 @@
 // clocks, the products 512 (D = 64) or 1024; for few rows the conversion and loads.
 // Measured (one B200): about 2800 clocks a tile, from the latency of a softmax warp's
 // chain (issue slots 50 % used, exponentials at 35 % of their rate, tensor pipe 16 %);
-// 8 chunks of 512 tokens over 3000 to 5000, 32 q / 4 kv heads of 64, INT8: 428 us a
-// layer, 334 TFLOP/s; 64 contexts U[128, 2048] with trees of 16, INT4: 80 us a layer,
-// of which some 15 are the prologue, first tile, drafted tile and join.
+// 8 chunks of 512 tokens over 3000 to 5000, 32 q / 4 kv heads of 64, INT8: 427 us a
+// layer, 335 TFLOP/s, 1.7 us of an SM per tile.  Short items are dearer, since the
+// registers leave room for one CTA per SM and nothing runs beside its prologue, first
+// conversion and epilogue: 64 contexts U[128, 2048] with trees of 16, INT4, are 388
+// items of 6.7 tiles, 79 us a layer, 4.5 us of an SM per tile.
 #pragma once
 
 #include "mg_tcgen05.cuh"
